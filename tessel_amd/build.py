@@ -21,6 +21,10 @@ HIP_FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-Wall", "-
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-mf16c"]  # f16 conversions in hardware
 
+# gemm_i8.hip: MFMA accumulators in VGPRs. With a register budget above 256 the
+# compiler put them in AGPRs and copied all of them once a K step.
+FILE_FLAGS = {"gemm_i8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+
 SOURCES = ["runtime.hip", "gemm.hip", "attention.hip", "decode.hip", "rows.hip", "quant_rows.hip", "gemm_i8.hip",
            "decode_q4.hip", "probe.hip"]
 HOST_SOURCES = ["engine.cpp", "checkpoint.cpp"]
@@ -41,7 +45,7 @@ def build(verbose=False):
     for s in SOURCES:
         o = os.path.join(BUILD, s.replace(".hip", ".o"))
         objs.append(o)
-        jobs.append([HIPCC] + HIP_FLAGS + ["-c", os.path.join(CSRC, s), "-o", o])
+        jobs.append([HIPCC] + HIP_FLAGS + FILE_FLAGS.get(s, []) + ["-c", os.path.join(CSRC, s), "-o", o])
     for s in HOST_SOURCES:
         o = os.path.join(BUILD, s.replace(".cpp", ".o"))
         objs.append(o)
@@ -92,7 +96,7 @@ def build_poisoned():
     for s in SOURCES:
         o = os.path.join(BUILD, s.replace(".hip", ".poison.o"))
         objs.append(o)
-        jobs.append([HIPCC] + HIP_FLAGS + ["-DTSL_POISON_LDS", "-c", os.path.join(CSRC, s), "-o", o])
+        jobs.append([HIPCC] + HIP_FLAGS + FILE_FLAGS.get(s, []) + ["-DTSL_POISON_LDS", "-c", os.path.join(CSRC, s), "-o", o])
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(jobs))) as ex:
         list(ex.map(_compile, jobs))
     objs += [os.path.join(BUILD, s.replace(".cpp", ".o")) for s in HOST_SOURCES]

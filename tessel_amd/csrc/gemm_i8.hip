@@ -13,6 +13,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 namespace {
 
@@ -56,41 +57,63 @@ TSL_DEV void tile_of(int bid, int nwg, int tiles_m, int tiles_n, int G, int& tm,
     tn = (pid % width) / rows;
 }
 
-// Any K and alignment: 16-byte loads at byte alignment into registers, then LDS.
-// Tiles of BM x BN products; gate_up's B tile holds, for each wavefront column, WN / 2 rows of
-// Wg and their partners of Wu, so a lane has both sums of an output.
-template <int EPI, int BM, int BN>
-__global__ __launch_bounds__(256) void gemm_i8_any(Gemm8 a) {
+// Any K and alignment: 16-byte loads at byte alignment into registers, a step ahead, then LDS.
+// 64 x 64 products a workgroup; KG groups of 4 wavefronts take steps g, g + KG, .. of 128 k
+// through two stages of their own, and their sums are added through LDS at the end (4 groups
+// where the tiles make one round on the CUs, else 2: 33 x 2049 x 4095 16.5 / 18.5 us).
+// gate_up's tile holds, for each wavefront column, WN / 2 rows of Wg and their partners of
+// Wu, so a lane has both sums of an output. A chunk that crosses its row's end is the row's last 16 bytes,
+// shifted, so that nothing past a row is read.
+//
+// Bound by the loads, which straddle lines: 777 x 1155 x 1001 9.5 us (12.5 with one group and each
+// step's loads waited for), 4001 x 4001 x 1001 95.
+template <int EPI, int KG>
+__global__ __launch_bounds__(256 * KG) void gemm_i8_any(Gemm8 a) {
     constexpr bool DUAL = EPI == Q_SWIGLU;
+    constexpr int BM = 64, BN = 64;
     constexpr int BK = 128, KC = BK / 16;                   // bytes and 16-byte chunks of a tile row
     constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
     constexpr int CA = BM * KC / 256, CB = BN * KC / 256;   // chunks a thread
     constexpr int OUT = DUAL ? BN / 2 : BN;                 // columns of Y a tile
-    __shared__ __attribute__((aligned(16))) u32x4 lds[(BM + BN) * KC];
+    constexpr int STAGE = (BM + BN) * KC;
+    __shared__ __attribute__((aligned(16))) u32x4 lds[KG * 2 * STAGE];
     TSL_POISON(lds);
     auto sw = [](int r) { return (r >> 1) & 7; };
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = threadIdx.x;
-    const int wm0 = (wave >> 1) * WM, wn0 = (wave & 1) * WN;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = threadIdx.x & 255;
+    const int kg = wave >> 2, w4 = wave & 3;
+    const int wm0 = (w4 >> 1) * WM, wn0 = (w4 & 1) * WN;
     int tm, tn;
     tile_of(blockIdx.x, gridDim.x, (a.M + BM - 1) / BM, (a.N + OUT - 1) / OUT, 8, tm, tn);
-    const int m0 = tm * BM, n0 = tn * OUT;
+    const int m0 = tm * BM, n0 = tn * OUT, K = a.K;
+    u32x4* ring = lds + kg * 2 * STAGE;
     // Tile row r of B: the row of W (or Wu) it holds.
     auto brow = [&](int r) -> const int8_t* {
-        if constexpr (!DUAL) return a.W + (size_t)min(n0 + r, a.N - 1) * a.K;
+        if constexpr (!DUAL) return a.W + (size_t)min(n0 + r, a.N - 1) * K;
         const int j = r % WN, n = n0 + (r / WN) * (WN / 2) + j % (WN / 2);
-        return (j < WN / 2 ? a.W : a.W2) + (size_t)min(n, a.N - 1) * a.K;
+        return (j < WN / 2 ? a.W : a.W2) + (size_t)min(n, a.N - 1) * K;
     };
     const int8_t *pa[CA], *pb[CB];
+    const int c16 = 16 * (t % KC);  // this thread's chunk of every row it loads
 #pragma unroll
-    for (int i = 0; i < CA; i++) pa[i] = a.X + (size_t)min(m0 + (i * 256 + t) / KC, a.M - 1) * a.K;
+    for (int i = 0; i < CA; i++) pa[i] = a.X + (size_t)min(m0 + (i * 256 + t) / KC, a.M - 1) * K;
 #pragma unroll
     for (int i = 0; i < CB; i++) pb[i] = brow((i * 256 + t) / KC);
     auto chunk = [&](const int8_t* row, int k) {  // 16 k of a row from k on, zeros past K
-        if (k + 16 <= a.K) return (u32x4) * reinterpret_cast<const u32x4b*>(row + k);
+        if (k + 16 <= K) return (u32x4) * reinterpret_cast<const u32x4b*>(row + k);
         u32x4 v = {0, 0, 0, 0};
+        if (k >= K) return v;
+        if (K >= 16) {
+            typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+            u64x2 q = __builtin_bit_cast(u64x2, (u32x4) * reinterpret_cast<const u32x4b*>(row + K - 16));
+            const int drop = 8 * (k + 16 - K);  // (8 .. 120 bits: the chunk starts at a multiple of 16)
+            if (drop >= 64) q = u64x2{q[1], 0};
+            const int d = drop & 63;
+            if (d) q = u64x2{q[0] >> d | q[1] << (64 - d), q[1] >> d};
+            return __builtin_bit_cast(u32x4, q);
+        }
 #pragma unroll
-        for (int e = 0; e < 16; e++)
-            if (k + e < a.K) v[e >> 2] |= (uint32_t)(uint8_t)row[k + e] << (8 * (e & 3));
+        for (int e = 0; e < 15; e++)
+            if (k + e < K) v[e >> 2] |= (uint32_t)(uint8_t)row[k + e] << (8 * (e & 3));
         return v;
     };
     i32x4 acc[TM][TN];
@@ -99,43 +122,71 @@ __global__ __launch_bounds__(256) void gemm_i8_any(Gemm8 a) {
 #pragma unroll
         for (int j = 0; j < TN; j++) acc[i][j] = i32x4{};
     const int l16 = lane & 15, g16 = lane >> 4;
-    for (int k0 = 0; k0 < a.K; k0 += BK) {
-        u32x4 ra[CA], rb[CB];
+    const int rounds = ((K + BK - 1) / BK + KG - 1) / KG;  // (a group past the end multiplies zeros)
+    u32x4 ra[CA], rb[CB];
+    auto gload = [&](int round) {
+        const int k = (round * KG + kg) * BK + c16;
 #pragma unroll
-        for (int i = 0; i < CA; i++) ra[i] = chunk(pa[i], k0 + 16 * ((i * 256 + t) % KC));
+        for (int i = 0; i < CA; i++) ra[i] = chunk(pa[i], k);
 #pragma unroll
-        for (int i = 0; i < CB; i++) rb[i] = chunk(pb[i], k0 + 16 * ((i * 256 + t) % KC));
-        __syncthreads();
+        for (int i = 0; i < CB; i++) rb[i] = chunk(pb[i], k);
+    };
+    auto sstore = [&](int stage) {
+        u32x4* s = ring + stage * STAGE;
 #pragma unroll
         for (int i = 0; i < CA; i++) {
-            const int r = (i * 256 + t) / KC, c = (i * 256 + t) % KC;
-            lds[r * KC + (c ^ sw(r))] = ra[i];
+            const int r = (i * 256 + t) / KC;
+            s[r * KC + ((t % KC) ^ sw(r))] = ra[i];
         }
 #pragma unroll
         for (int i = 0; i < CB; i++) {
-            const int r = (i * 256 + t) / KC, c = (i * 256 + t) % KC;
-            lds[BM * KC + r * KC + (c ^ sw(r))] = rb[i];
+            const int r = (i * 256 + t) / KC;
+            s[BM * KC + r * KC + ((t % KC) ^ sw(r))] = rb[i];
         }
-        __syncthreads();
+    };
+    if (rounds > 0) {
+        gload(0);
+        sstore(0);
+    }
+    for (int q = 0; q < rounds; q++) {
+        __syncthreads();  // stage q is written, and every read of the other is done
+        if (q + 1 < rounds) gload(q + 1);
+        const u32x4* s = ring + (q & 1) * STAGE;
 #pragma unroll
         for (int st = 0; st < BK / 64; st++) {
             i32x4 av[TM], bv[TN];
 #pragma unroll
             for (int i = 0; i < TM; i++) {
                 const int r = wm0 + i * 16 + l16;
-                av[i] = __builtin_bit_cast(i32x4, lds[r * KC + ((4 * st + g16) ^ sw(r))]);
+                av[i] = __builtin_bit_cast(i32x4, s[r * KC + ((4 * st + g16) ^ sw(r))]);
             }
 #pragma unroll
             for (int j = 0; j < TN; j++) {
                 const int r = wn0 + j * 16 + l16;
-                bv[j] = __builtin_bit_cast(i32x4, lds[BM * KC + r * KC + ((4 * st + g16) ^ sw(r))]);
+                bv[j] = __builtin_bit_cast(i32x4, s[BM * KC + r * KC + ((4 * st + g16) ^ sw(r))]);
             }
 #pragma unroll
             for (int i = 0; i < TM; i++)
 #pragma unroll
                 for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[i], bv[j], acc[i][j], 0, 0, 0);
         }
+        if (q + 1 < rounds) sstore((q + 1) & 1);
     }
+    __syncthreads();
+    i32x4* red = reinterpret_cast<i32x4*>(lds);  // [KG - 1][4 wavefronts][TM TN][64]
+    if (kg > 0)
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int j = 0; j < TN; j++) red[(((kg - 1) * 4 + w4) * TM * TN + i * TN + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll
+    for (int g = 0; g < KG - 1; g++)
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int j = 0; j < TN; j++) acc[i][j] += red[((g * 4 + w4) * TM * TN + i * TN + j) * 64 + lane];
     // Lane l of a 16 x 16 tile: column l % 16, rows 4 (l / 16) + r.
     constexpr int TNO = DUAL ? TN / 2 : TN;
 #pragma unroll
@@ -157,12 +208,545 @@ __global__ __launch_bounds__(256) void gemm_i8_any(Gemm8 a) {
     }
 }
 
+// ---------------------------------------------------------------- aligned rows
+// K % 16 == 0 and 16-byte aligned operands: tiles go from global memory into LDS by
+// direct buffer loads of 8 rows x 128 bytes (lane i of a load lands at the load's LDS base + 16 i,
+// so the swizzle is in which chunk each lane fetches); the resources
+// begin at the tile's first row, so operands may be of any size, and rows past the operand's end
+// read as zero.
+//
+// W is the MFMA's A operand and X its B operand, so a lane ends with 4
+// consecutive columns of one row of Y a tile; and the rows of W that tile j
+// of a wavefront holds are 4 of every 4 TN: row 4 g + r of tile j is W row
+// 4 TN g + 4 j + r, so that a lane's tiles together are 4 TN consecutive
+// columns, stored 16 bytes at a time. gate_up's wavefronts hold WN / 2
+// rows of Wg and the same of Wu, tile by tile, so a lane has both sums of an output.
+typedef __attribute__((address_space(3))) void lds_void_t;
+constexpr int OOB = 0x7fffffff;  // a byte offset past any range
+
+// s_waitcnt immediate for vmcnt(n) alone (6-bit vmcnt: bits 3:0 and 15:14).
+constexpr int vmcnt_imm(int n) { return (n & 15) | ((n >> 4) << 14) | 0x0f70; }
+
+TSL_DEV i32x4 make_rsrc(const void* p, uint32_t bytes) {
+    const uint64_t a = reinterpret_cast<uint64_t>(p);
+    return i32x4{(int)(uint32_t)a, (int)(uint32_t)((a >> 32) & 0xffff), (int)bytes, 0x00020000};
+}
+
+TSL_DEV void load_lds(uint32_t dst, uint32_t off, const i32x4& rs) {
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(dst), "v"(off), "s"(rs) : "memory");
+}
+
+// Stores a lane's outputs: row m of Y, CNT consecutive columns from n.
+template <int CNT>
+TSL_DEV void store_cols(u16* Y, int N, int m, int n, const u16 (&v)[CNT]) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    typedef u32x4 u32x4h __attribute__((aligned(2)));
+    typedef u32x2 u32x2h __attribute__((aligned(2)));
+    u16* y = Y + (size_t)m * N + n;
+    if (n + CNT <= N) {
+        uint32_t w[CNT / 2];
+#pragma unroll
+        for (int i = 0; i < CNT / 2; i++) w[i] = (uint32_t)v[2 * i] | (uint32_t)v[2 * i + 1] << 16;
+        if constexpr (CNT % 8 == 0)
+#pragma unroll
+            for (int i = 0; i < CNT / 8; i++)
+                *reinterpret_cast<u32x4h*>(y + 8 * i) = u32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
+        else
+#pragma unroll
+            for (int i = 0; i < CNT / 4; i++) *reinterpret_cast<u32x2h*>(y + 4 * i) = u32x2{w[2 * i], w[2 * i + 1]};
+    } else {
+#pragma unroll
+        for (int i = 0; i < CNT; i++)
+            if (n + i < N) y[i] = v[i];
+    }
+}
+
+// The epilogue of a wavefront's TM x TN tiles: rows m0 + 16 i + l % 16 of Y,
+// columns n0 + 4 TNO (l / 16) .. (TNO: tiles of outputs).
+template <int EPI, int TM, int TN>
+TSL_DEV void store_tiles(const Gemm8& a, int m0, int n0, int lane, const i32x4 (&acc)[TM][TN]) {
+    constexpr bool DUAL = EPI == Q_SWIGLU;
+    constexpr int TNO = DUAL ? TN / 2 : TN, CNT = 4 * TNO;
+    const int n = n0 + CNT * (lane >> 4);
+    if (n >= a.N) return;
+    float sw[CNT], su[DUAL ? CNT : 1];
+#pragma unroll
+    for (int c = 0; c < CNT; c++) {
+        sw[c] = a.SW[min(n + c, a.N - 1)];
+        if constexpr (DUAL) su[c] = a.SW2[min(n + c, a.N - 1)];
+    }
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+        const int m = m0 + 16 * i + (lane & 15);
+        if (m >= a.M) continue;
+        const float sx = a.SX[m];
+        u16 v[CNT];
+#pragma unroll
+        for (int c = 0; c < CNT; c++) {
+            float f = scaled(acc[i][c / 4][c % 4], sx, sw[c]);
+            if constexpr (DUAL) f = silu_mul(f, scaled(acc[i][TNO + c / 4][c % 4], sx, su[c]));
+            v[c] = f2h(f);
+        }
+        store_cols<CNT>(a.Y, a.N, m, n, v);
+    }
+}
+
+// Swizzles of a tile's rows (8 chunks of 16 bytes each): chunk c of row r sits
+// at c ^ sw(r), so that the 16 rows of an operand read cover all 16 positions of
+// LDS's 256-byte bank window. X reads rows 16 i + l; W (TNO tiles of outputs a wavefront)
+// rows 4 TNO (l / 4) + 4 j + l % 4.
+TSL_DEV int swx(int r) { return (r >> 1) & 7; }
+template <int TNO>
+TSL_DEV int sww(int r) { return ((r >> 1) & 1) | (((r / (4 * TNO)) & 3) << 1); }
+
+// Where row r of the W tile comes from: the local output column, and whether it is Wu's.
+template <bool DUAL, int WN>
+TSL_DEV int w_row(int r) { return DUAL ? (r / WN) * (WN / 2) + r % (WN / 2) : r; }
+template <bool DUAL, int WN>
+TSL_DEV bool w_up(int r) { return DUAL && r % WN >= WN / 2; }
+
+// BM x BN tiles, WGM x WGN wavefronts, NS stages of 128 k in a ring. KG groups of wavefronts with a
+// ring each take steps g, g + KG, ..; their sums are added through LDS at the end.
+template <int EPI, int BM, int BN, int WGM, int WGN, int NS, int KG>
+__global__ __launch_bounds__(WGM* WGN* KG * 64, 1) void gemm_i8_tile(Gemm8 a) {
+    constexpr bool DUAL = EPI == Q_SWIGLU;
+    constexpr int BK = 128, NW = WGM * WGN;
+    constexpr int WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16, TNO = DUAL ? TN / 2 : TN;
+    constexpr int OUT = DUAL ? BN / 2 : BN;
+    constexpr int LPA = BM / 8 / NW, LPB = BN / 8 / NW, LPS = LPA + LPB;  // 1 KB loads a wavefront a step
+    static_assert(BM / 8 % NW == 0 && BN / 8 % NW == 0 && TM >= 1 && TNO >= 1, "tile shape");
+    constexpr int STAGE = (BM + BN) * BK;
+    static_assert(KG == 1 || (KG - 1) * BM * BN * 4 <= KG * NS * STAGE, "the reduction fits the rings");
+    __shared__ __attribute__((aligned(16))) char lds[KG * NS * STAGE];
+    TSL_POISON(lds);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int kg = wave / NW, w = wave % NW;
+    const int wm0 = (w / WGN) * WM, wn0 = (w % WGN) * WN;
+    int tm, tn;
+    tile_of(blockIdx.x, gridDim.x, (a.M + BM - 1) / BM, (a.N + OUT - 1) / OUT, 8, tm, tn);
+    const int m0 = tm * BM, n0 = tn * OUT, K = a.K;
+    char* ring = lds + kg * NS * STAGE;
+    const uint32_t ring_at = (uint32_t)reinterpret_cast<uintptr_t>((lds_void_t*)lds) + kg * NS * STAGE;
+    const uint32_t xbytes = (uint32_t)min(BM, a.M - m0) * K, wbytes = (uint32_t)min(OUT, a.N - n0) * K;
+    const int8_t *Xt = a.X + (size_t)m0 * K, *Wt = a.W + (size_t)n0 * K, *Wt2 = DUAL ? a.W2 + (size_t)n0 * K : Wt;
+
+    uint32_t offa[LPA], offb[LPB];
+    int ka[LPA], kb[LPB];
+#pragma unroll
+    for (int i = 0; i < LPA; i++) {
+        const int r = 8 * (w * LPA + i) + (lane >> 3), c = (lane & 7) ^ swx(r);
+        ka[i] = 16 * c;
+        offa[i] = (uint32_t)r * K + 16 * c;
+    }
+#pragma unroll
+    for (int i = 0; i < LPB; i++) {
+        const int r = 8 * (w * LPB + i) + (lane >> 3), c = (lane & 7) ^ sww<TNO>(r);
+        kb[i] = 16 * c;
+        offb[i] = (uint32_t)w_row<DUAL, WN>(r) * K + 16 * c;
+    }
+    // A step's loads into a stage: aim, then load 0 .. LPS - 1 (X's, then W's). Past K (the
+    // end of the last step; whole steps of a group that has one less) zeros are loaded.
+    i32x4 rx, rw, ru;
+    uint32_t dst;
+    int kleft;
+    auto aim = [&](int step, int stage) {
+        const int k0 = step * BK;
+        kleft = K - k0;
+        const uint32_t skip = min(k0, K);
+        rx = make_rsrc(Xt + skip, kleft > 0 ? xbytes - skip : 0);
+        rw = make_rsrc(Wt + skip, kleft > 0 ? wbytes - skip : 0);
+        ru = DUAL ? make_rsrc(Wt2 + skip, kleft > 0 ? wbytes - skip : 0) : rw;
+        dst = ring_at + stage * STAGE;
+    };
+    auto load = [&](int i) {
+        if (i < LPA) load_lds(dst + (w * LPA + i) * 1024, ka[i] < kleft ? offa[i] : (uint32_t)OOB, rx);
+        else load_lds(dst + BM * BK + (w * LPB + i - LPA) * 1024, kb[i - LPA] < kleft ? offb[i - LPA] : (uint32_t)OOB,
+                      w_up<DUAL, WN>(8 * (w * LPB + i - LPA)) ? ru : rw);
+    };
+    const int l16 = lane & 15, g16 = lane >> 4;
+    const int xr = wm0 + l16, wr = wn0 + 4 * TNO * (l16 >> 2) + (l16 & 3);  // tile 0's operand rows
+    auto x_at = [&](int st, int i) { return (uint32_t)((xr + 16 * i) * BK + (((4 * st + g16) ^ swx(xr)) * 16)); };
+    auto w_at = [&](int st, int j) {
+        const int r = wr + (j / TNO) * (WN / 2) + 4 * (j % TNO);
+        return (uint32_t)(BM * BK + r * BK + (((4 * st + g16) ^ sww<TNO>(r)) * 16));
+    };
+    i32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) acc[i][j] = i32x4{};
+
+    // The ring, software pipelined: step t's second 64 k are read from LDS under its
+    // first 64 k's MFMAs, and the next step's first under its second's. Between the
+    // two every wavefront holds all of step t in registers and step t + 1 has landed (the
+    // barrier), so step t's stage is loaded again, NS - 1 steps ahead. Reads and loads are
+    // dealt out between the MFMAs: a wavefront issues in order, and a burst of
+    // either would hold the MFMAs behind it.
+    const int nsteps = (K + BK - 1) / BK, rounds = (nsteps + KG - 1) / KG;
+    constexpr int NM = TM * TN, NR = TM + TN;
+    i32x4 xa[TM], wa[TN], xb[TM], wb[TN];
+    auto read = [&](int stage, int st, i32x4 (&x)[TM], i32x4 (&v)[TN], int r) {  // the r-th of NR
+        const char* sp = ring + stage * STAGE;
+        if (r < TN) v[r] = *reinterpret_cast<const i32x4*>(sp + w_at(st, r));
+        else x[r - TN] = *reinterpret_cast<const i32x4*>(sp + x_at(st, r - TN));
+    };
+    auto half = [&](const i32x4 (&x)[TM], const i32x4 (&v)[TN], auto reads, auto loads, int nread, int nload) {
+#pragma unroll
+        for (int q = 0; q < NM; q++) {
+            acc[q / TN][q % TN] = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[q % TN], x[q / TN], acc[q / TN][q % TN], 0, 0, 0);
+#pragma unroll
+            for (int r = q * nread / NM; r < (q + 1) * nread / NM; r++) reads(r);
+#pragma unroll
+            for (int r = q * nload / NM; r < (q + 1) * nload / NM; r++) loads(r);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    for (int p = 0; p < NS && p < rounds; p++) {
+        aim(p * KG + kg, p);
+#pragma unroll
+        for (int i = 0; i < LPS; i++) load(i);
+    }
+    if (rounds >= NS) __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 1) * LPS));
+    else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < NR; r++) read(0, 0, xa, wa, r);
+    int stage = 0;
+    auto none = [](int) {};
+    auto step = [&](int t, auto more) {
+        constexpr bool MORE = decltype(more)::value;
+        const int next = stage + 1 == NS ? 0 : stage + 1;
+        half(xa, wa, [&](int r) { read(stage, 1, xb, wb, r); }, none, NR, 0);
+        __builtin_amdgcn_s_waitcnt(MORE ? vmcnt_imm((NS - 2) * LPS) : vmcnt_imm(0));
+        __syncthreads();
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (MORE) {
+            aim((t + NS) * KG + kg, stage);
+            half(xb, wb, [&](int r) { read(next, 0, xa, wa, r); }, load, NR, LPS);
+        } else {
+            half(xb, wb, [&](int r) { read(next, 0, xa, wa, r); }, none, NR, 0);
+        }
+        stage = next;
+    };
+    int t = 0;
+    for (; t + NS < rounds; t++) step(t, std::integral_constant<bool, true>{});
+    for (; t + 1 < rounds; t++) step(t, std::integral_constant<bool, false>{});
+    half(xa, wa, [&](int r) { read(stage, 1, xb, wb, r); }, none, NR, 0);
+    half(xb, wb, none, none, 0, 0);
+    if constexpr (KG > 1) {
+        i32x4* red = reinterpret_cast<i32x4*>(lds);  // [KG - 1][NW][TM TN][64]
+        __syncthreads();
+        if (kg > 0)
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+#pragma unroll
+                for (int j = 0; j < TN; j++) red[(((kg - 1) * NW + w) * TM * TN + i * TN + j) * 64 + lane] = acc[i][j];
+        __syncthreads();
+        if (kg > 0) return;
+#pragma unroll
+        for (int g = 0; g < KG - 1; g++)
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+#pragma unroll
+                for (int j = 0; j < TN; j++) acc[i][j] += red[((g * NW + w) * TM * TN + i * TN + j) * 64 + lane];
+    }
+    store_tiles<EPI, TM, TN>(a, m0 + wm0, n0 + (DUAL ? wn0 / 2 : wn0), lane, acc);
+}
+
+// Large products (K % 128 == 0): 256 x 256 tiles as a ping-pong of two groups of
+// 4 wavefronts, one of each on every SIMD, in turns between workgroup barriers:
+// while one group's MFMAs run back to back from registers, the other reads
+// its next step's operands from LDS. gemm_pp16's phases and stages (two of X,
+// loaded by group 0; three of W, loaded by group 1 two steps ahead: 160 KB), with 128 k a step.
+template <int EPI>
+__global__ __launch_bounds__(512, 1) void gemm_i8_pp(Gemm8 a) {
+    constexpr bool DUAL = EPI == Q_SWIGLU;
+    constexpr int BM = 256, BK = 128;
+    constexpr int WM = 128, WN = 64, TM = 8, TN = 4, TNO = DUAL ? 2 : 4, OUT = DUAL ? 128 : 256;
+    constexpr int LP = 8;             // 1 KB loads a wavefront a step
+    constexpr int TILE = BM * BK;     // bytes of a stage of X (or W)
+    constexpr int WBASE = 2 * TILE;
+    __shared__ __attribute__((aligned(16))) char lds[5 * TILE];
+    TSL_POISON(lds);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int grp = wave >> 2, w4 = wave & 3;
+    const int wm0 = grp * WM, wn0 = w4 * WN;
+    int tm, tn;
+    tile_of(blockIdx.x, gridDim.x, (a.M + BM - 1) / BM, (a.N + OUT - 1) / OUT, 4, tm, tn);
+    const int m0 = tm * BM, n0 = tn * OUT, K = a.K;
+    const int l16 = lane & 15, g16 = lane >> 4;
+    const uint32_t lds_at = (uint32_t)reinterpret_cast<uintptr_t>((lds_void_t*)lds);
+    const uint32_t xbytes = (uint32_t)min(BM, a.M - m0) * K, wbytes = (uint32_t)min(OUT, a.N - n0) * K;
+    const int8_t *Xt = a.X + (size_t)m0 * K, *Wt = a.W + (size_t)n0 * K, *Wt2 = DUAL ? a.W2 + (size_t)n0 * K : Wt;
+
+    uint32_t off[LP];
+#pragma unroll
+    for (int i = 0; i < LP; i++) {
+        const int r = 8 * (w4 * LP + i) + (lane >> 3);
+        off[i] = grp == 0 ? (uint32_t)r * K + 16 * ((lane & 7) ^ swx(r))
+                          : (uint32_t)w_row<DUAL, WN>(r) * K + 16 * ((lane & 7) ^ sww<TNO>(r));
+    }
+    auto issue = [&](int step, int stage) {
+        const int k0 = step * BK;
+        auto uniform = [](i32x4 v) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) v[c] = __builtin_amdgcn_readfirstlane(v[c]);
+            return v;
+        };
+        const i32x4 r0 = uniform(grp == 0 ? make_rsrc(Xt + k0, xbytes - k0) : make_rsrc(Wt + k0, wbytes - k0));
+        const i32x4 r1 = uniform(grp == 0 ? r0 : make_rsrc(Wt2 + k0, wbytes - k0));
+        const uint32_t dst = __builtin_amdgcn_readfirstlane(lds_at + (grp == 0 ? 0 : WBASE) + stage * TILE + w4 * LP * 1024);
+#pragma unroll
+        for (int i = 0; i < LP; i++) load_lds(dst + i * 1024, off[i], DUAL && i >= LP / 2 ? r1 : r0);
+    };
+    static_assert(LP * 8 == WN, "a wavefront of group 1 loads its own rows of W: Wg's, then Wu's");
+    const int xr = wm0 + l16, wr = wn0 + 4 * TNO * (l16 >> 2) + (l16 & 3);
+    uint32_t x_at[2], w_at[2][TN];
+#pragma unroll
+    for (int st = 0; st < 2; st++) {
+        x_at[st] = (uint32_t)(xr * BK + (((4 * st + g16) ^ swx(xr)) * 16));
+#pragma unroll
+        for (int j = 0; j < TN; j++) {
+            const int r = wr + (j / TNO) * (WN / 2) + 4 * (j % TNO);
+            w_at[st][j] = (uint32_t)(WBASE + r * BK + (((4 * st + g16) ^ sww<TNO>(r)) * 16));
+        }
+    }
+    i32x4 xv[2][TM], wv[2][TN];
+    auto read_step = [&](int stage, int wstage) {
+#pragma unroll
+        for (int st = 0; st < 2; st++) {
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+                xv[st][i] = *reinterpret_cast<const i32x4*>(lds + stage * TILE + x_at[st] + i * 16 * BK);
+#pragma unroll
+            for (int j = 0; j < TN; j++) wv[st][j] = *reinterpret_cast<const i32x4*>(lds + wstage * TILE + w_at[st][j]);
+        }
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    i32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) acc[i][j] = i32x4{};
+    auto compute = [&]() {
+#pragma unroll
+        for (int st = 0; st < 2; st++)
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+#pragma unroll
+                for (int j = 0; j < TN; j++)
+                    acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[st][j], xv[st][i], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto bar = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const int nk = K / BK;
+    int ws = 0;  // W's stage of step s
+    issue(0, 0);
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    bar();
+    if (grp == 0) {
+        for (int s = 0; s < nk; s++) {
+            if (s + 1 < nk) issue(s + 1, (s + 1) & 1);
+            read_step(s & 1, ws);
+            bar();
+            compute();
+            ws = ws == 2 ? 0 : ws + 1;
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+            bar();
+        }
+    } else {
+        if (nk > 1) issue(1, 1);
+        bar();
+        for (int s = 0; s < nk; s++) {
+            read_step(s & 1, ws);
+            if (s + 2 < nk) {
+                issue(s + 2, ws == 0 ? 2 : ws - 1);
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(LP));
+            } else {
+                __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+            }
+            bar();
+            compute();
+            ws = ws == 2 ? 0 : ws + 1;
+            if (s + 1 < nk) bar();
+        }
+    }
+    store_tiles<EPI, TM, TN>(a, m0 + wm0, n0 + (DUAL ? wn0 / 2 : wn0), lane, acc);
+}
+
+// Few rows (M <= 64): a stream of W. A workgroup of 8 wavefronts has 16 rows of W
+// (gate_up: 8 of Wg and their 8 of Wu); wavefront w takes the 128-k steps w, w + 8, ..
+// through a ring of D stages of its own (W's 16 rows, X's 16 MT), whole 128-byte
+// lines a load, and waits for nobody's loads but its own. The 8 partial
+// tiles are added through LDS.
+template <int EPI, int MT, int D>
+__global__ __launch_bounds__(512) void gemm_i8_skinny(Gemm8 a) {
+    constexpr bool DUAL = EPI == Q_SWIGLU;
+    constexpr int NWV = 8, BK = 128, STAGE = (16 + 16 * MT) * BK, L = 2 + 2 * MT;  // loads a stage
+    constexpr int RING = NWV * D * STAGE, RED = NWV * MT * 1024;
+    __shared__ __attribute__((aligned(16))) char lds[RING > RED ? RING : RED];
+    TSL_POISON(lds);
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g16 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n0 = blockIdx.x * (DUAL ? 8 : 16), K = a.K;
+    const uint32_t wbytes = (uint32_t)min(DUAL ? 8 : 16, a.N - n0) * K, xbytes = (uint32_t)a.M * K;
+    const int8_t *Wt = a.W + (size_t)n0 * K, *Wt2 = DUAL ? a.W2 + (size_t)n0 * K : Wt;
+    char* ring = lds + wave * D * STAGE;
+    const uint32_t ring_at = (uint32_t)reinterpret_cast<uintptr_t>((lds_void_t*)lds) + wave * D * STAGE;
+    const int nsteps = (K + BK - 1) / BK, mine = nsteps > wave ? (nsteps - wave + NWV - 1) / NWV : 0;
+    auto issue = [&](int u, int stage) {
+        const int k0 = (wave + NWV * u) * BK;
+        const uint32_t at = ring_at + stage * STAGE;
+        const i32x4 rw = make_rsrc(Wt + k0, wbytes - k0), ru = make_rsrc(Wt2 + k0, wbytes - k0), rx = make_rsrc(a.X + k0, xbytes - k0);
+#pragma unroll
+        for (int i = 0; i < L; i++) {
+            const int r = 8 * (i < 2 ? i : i - 2) + (lane >> 3), c = (lane & 7) ^ swx(r);
+            const uint32_t off = (uint32_t)(DUAL && i < 2 ? r & 7 : r) * K + 16 * c;
+            load_lds(at + i * 1024, k0 + 16 * c < K ? off : (uint32_t)OOB, i >= 2 ? rx : DUAL && i == 1 ? ru : rw);
+        }
+    };
+    for (int u = 0; u < D && u < mine; u++) issue(u, u);
+    i32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; t++) acc[t] = i32x4{};
+    int stage = 0;
+    for (int u = 0; u < mine; u++) {
+        const int ahead = min(D - 1, mine - 1 - u);
+        if (ahead <= 0) __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+        else if (ahead == 1) __builtin_amdgcn_s_waitcnt(vmcnt_imm(L));
+        else __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * L));
+        asm volatile("" ::: "memory");
+        const char* sp = ring + stage * STAGE;
+        i32x4 wv[2], xv[2][MT];
+#pragma unroll
+        for (int st = 0; st < 2; st++) {
+            const int c = 16 * ((4 * st + g16) ^ swx(l16));
+            wv[st] = *reinterpret_cast<const i32x4*>(sp + l16 * BK + c);
+#pragma unroll
+            for (int t = 0; t < MT; t++) xv[st][t] = *reinterpret_cast<const i32x4*>(sp + (16 + 16 * t + l16) * BK + c);
+        }
+#pragma unroll
+        for (int st = 0; st < 2; st++)
+#pragma unroll
+            for (int t = 0; t < MT; t++) acc[t] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[st], xv[st][t], acc[t], 0, 0, 0);
+        // (the operands are in registers before their stage is loaded again)
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        asm volatile("" ::: "memory");
+        if (u + D < mine) issue(u + D, stage);
+        stage = stage + 1 == D ? 0 : stage + 1;
+    }
+    static_assert(D <= 3, "the waits above");
+    // Lane l: W rows 4 (l / 16) + r, row 16 t + l % 16 of X.
+    i32x4* red = reinterpret_cast<i32x4*>(lds);  // [MT][wavefront][64]
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < MT; t++) red[(t * NWV + wave) * 64 + lane] = acc[t];
+    __syncthreads();
+    // gate_up: lanes 0 .. 31 hold gate sums, 32 on their up partners.
+    for (int t = wave; t < MT; t += NWV) {
+        i32x4 s = {0, 0, 0, 0}, u = {0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < NWV; w++) {
+            s += red[(t * NWV + w) * 64 + lane];
+            if constexpr (DUAL) u += red[(t * NWV + w) * 64 + (lane | 32)];
+        }
+        const int m = 16 * t + l16, n = n0 + 4 * g16;
+        if (m >= a.M || n >= a.N || (DUAL && g16 >= 2)) continue;
+        const float sx = a.SX[m];
+        u16 v[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int nn = min(n + r, a.N - 1);
+            float f = scaled(s[r], sx, a.SW[nn]);
+            if constexpr (DUAL) f = silu_mul(f, scaled(u[r], sx, a.SW2[nn]));
+            v[r] = f2h(f);
+        }
+        store_cols<4>(a.Y, a.N, m, n, v);
+    }
+}
+
+template <int EPI, int BM, int BN, int WGM, int WGN, int NS, int KG>
+int run_tile(const Gemm8& a, hipStream_t s) {
+    constexpr int OUT = EPI == Q_SWIGLU ? BN / 2 : BN;
+    const long tiles = (long)((a.M + BM - 1L) / BM) * ((a.N + OUT - 1L) / OUT);
+    hipLaunchKernelGGL((gemm_i8_tile<EPI, BM, BN, WGM, WGN, NS, KG>), dim3((unsigned)tiles), dim3(WGM * WGN * KG * 64), 0, s, a);
+    return TSL_LAUNCHED("quant product");
+}
+
+// The time of a product by each form, in us, from its LDS traffic, which bounds
+// them all (128 bytes a clock and CU; a larger tile reads each staged row more often):
+// a step of 128 k costs what it measured on one busy CU, 0.4 of it more with all CUs busy
+// (the clock falls), and a product takes as many rounds of them as its tiles need on the CUs:
+//   64 x 64 .18 us, 64 x 128 .26, 128 x 128 .37, 256 x 128 .60, 256 x 256 .91, and 3 to 6 us for
+// filling, the epilogue and the launch. The skinny form stages 16 rows of W and all of X a block, 54 KB
+// a us and CU. Measured / chosen by this, us: linear 65 x 2048 x 5632 64 x 64 10.9
+// (256 x 256 44.8), 512 x 4096 x 4096 64 x 128 13.6 (64 x 64 18.0, 128 x 128 17.1), 1024 x 4096
+// x 4096 128 x 128 20.7 (256 x 128 26.6), gate_up 512 x 5632 x 2048 256 x 128 16.6 (128 x 128
+// 21.2, 256 x 256 24.6), linear 4096 x 4096 x 4096 256 x 256 54.2 (256 x 128 68.6);
+// gate_up 32 x 11008 x 4096 64 x 128 16.3 (skinny 22.8), 1 x 5632 x 2048 skinny 4.9 (64 x 64 5.9), linear
+// 64 x 2048 x 5632 skinny 6.2 (64 x 64 10.8).
+struct Form {
+    double step, fixed;
+    int bm, out;
+};
+double form_cost(const Form& f, const Gemm8& a) {
+    const double tiles = (double)((a.M + f.bm - 1) / f.bm) * ((a.N + f.out - 1) / f.out), cus = num_cus();
+    const double rounds = std::max(1.0, (double)(long)((tiles + cus - 1) / cus)), steps = (a.K + 127) / 128;
+    return f.fixed + rounds * steps * f.step * (1.0 + 0.4 * tiles / (rounds * cus));
+}
+
+template <int EPI, int MT, int D>
+int run_skinny(const Gemm8& a, hipStream_t s) {
+    constexpr int ROWS = EPI == Q_SWIGLU ? 8 : 16;
+    hipLaunchKernelGGL((gemm_i8_skinny<EPI, MT, D>), dim3((unsigned)((a.N + ROWS - 1) / ROWS)), dim3(512), 0, s, a);
+    return TSL_LAUNCHED("quant product");
+}
+
 template <int EPI>
 int run_gemm8(const Gemm8& a, hipStream_t s) {
     if (a.M == 0 || a.N == 0) return 0;
-    constexpr int OUT = EPI == Q_SWIGLU ? 32 : 64;
-    const long tiles = (long)((a.M + 63L) / 64) * ((a.N + OUT - 1L) / OUT);
-    hipLaunchKernelGGL((gemm_i8_any<EPI, 64, 64>), dim3((unsigned)tiles), dim3(256), 0, s, a);
+    constexpr int HALF = EPI == Q_SWIGLU ? 2 : 1;  // gate_up's tiles hold two rows of W a column
+    if (((uint64_t)a.X | (uint64_t)a.W | (uint64_t)a.W2 | (uint64_t)a.K) % 16 != 0 || a.K == 0) {
+        const long tiles = (long)((a.M + 63L) / 64) * ((a.N + 64 / HALF - 1L) / (64 / HALF));
+        if (tiles <= num_cus()) hipLaunchKernelGGL((gemm_i8_any<EPI, 4>), dim3((unsigned)tiles), dim3(1024), 0, s, a);
+        else hipLaunchKernelGGL((gemm_i8_any<EPI, 2>), dim3((unsigned)tiles), dim3(512), 0, s, a);
+        return TSL_LAUNCHED("quant product");
+    }
+    const Form forms[] = {{0.18, 2.8, 64, 64 / HALF},    {0.26, 3.2, 64, 128 / HALF},   {0.37, 4.0, 128, 128 / HALF},
+                          {0.60, 4.2, 256, 128 / HALF}, {0.91, 6.0, 256, 256 / HALF}};
+    int pick = 0;
+    double best = form_cost(forms[0], a);
+    for (int i = 1; i < 5; i++) {
+        const double c = form_cost(forms[i], a);
+        if (c < best && (i < 4 || a.K % 128 == 0)) pick = i, best = c;
+    }
+    const int mt = (a.M + 15) / 16;
+    if (mt <= 4) {
+        const double blocks = (a.N + 16 / HALF - 1) / (16 / HALF), kb = (16.0 + 16 * mt) * a.K / 1024;
+        if (2.0 + std::max(1.0, blocks / num_cus()) * kb / 54 < best) {
+            switch (mt) {
+                case 1: return run_skinny<EPI, 1, 2>(a, s);
+                case 2: return run_skinny<EPI, 2, 3>(a, s);
+                case 3: return run_skinny<EPI, 3, 2>(a, s);
+                default: return run_skinny<EPI, 4, 2>(a, s);
+            }
+        }
+    }
+    switch (pick) {
+        case 0: return run_tile<EPI, 64, 64, 2, 2, 4, 2>(a, s);
+        case 1: return run_tile<EPI, 64, 128, 2, 2, 3, 2>(a, s);
+        case 2: return run_tile<EPI, 128, 128, 2, 4, 4, 1>(a, s);
+        case 3: return run_tile<EPI, 256, 128, 4, 2, 3, 1>(a, s);
+    }
+    const long tiles = (long)((a.M + 255L) / 256) * ((a.N + 256 / HALF - 1L) / (256 / HALF));
+    hipLaunchKernelGGL(gemm_i8_pp<EPI>, dim3((unsigned)tiles), dim3(512), 0, s, a);
     return TSL_LAUNCHED("quant product");
 }
 
@@ -171,6 +755,8 @@ int check_i8(const TslKernel& k, const char* n) {
         return tsl_fail(-2, "quant/" + k.name + ": K = " + std::to_string(k.dim("K")) + " exceeds 131071 (sums of 8-bit products in 32 bits)");
     if (k.dim("M") > (1 << 24) || k.dim(n) > (1 << 24))
         return tsl_fail(-2, "quant/" + k.name + ": at most 2^24 rows and columns");
+    // (a launch holds 2^32 work-items; 512 of them make 64 x 32 outputs at least)
+    if ((k.dim("M") + 63) * (k.dim(n) + 31) > (1LL << 34)) return tsl_fail(-2, "quant/" + k.name + ": at most 2^34 outputs");
     return 0;
 }
 

@@ -31,6 +31,7 @@ def _write(t=3, w=768, g=2, d=64, p=16, **kw):
     ("linear", [[2, 64], [3], [3, 64], [3], [2, 3]], "dimension M is 2 and 3"),
     ("linear", [[2, 64], [2], [3, 64], [3], [2, 4]], "dimension N is 3 and 4"),
     ("linear", [[2 ** 25, 64], [2 ** 25], [3, 64], [3], [2 ** 25, 3]], "at most 2\\^24"),
+    ("linear", [[2 ** 18, 64], [2 ** 18], [2 ** 18, 64], [2 ** 18], [2 ** 18, 2 ** 18]], "at most 2\\^34 outputs"),
     ("gate_up", [[2, 131072], [2], [3, 131072], [3], [3, 131072], [3], [2, 3]], "K = 131072 exceeds"),
     ("gate_up", [[2, 64], [2], [3, 64], [3], [4, 64], [4], [2, 3]], "dimension F is 3 and 4"),
     ("quantize", [[2, 64], [2, 64], [3]], "dimension M is 2 and 3"),
