@@ -29,7 +29,8 @@ struct Q4Args {
     u16* O;
     float* part;  // [B][G][NCH][QPG][2 + D]: m, l, acc
     int B, H, G, NP, P, MP, NCH;
-    int CT;       // tokens per chunk
+    int CT;       // tokens per chunk (a multiple of 256)
+    int pshift;   // log2(P)
     float c2;     // scale log2(e)
 };
 
@@ -52,12 +53,15 @@ __global__ __launch_bounds__(256) void decode_q4_any(Q4Args a) {
     __shared__ float mrun[QPG], lrun[QPG], keep[QPG], lowsum[QPG], part[4][QPG][2], red[NG][D];
     TSL_POISON(qs); TSL_POISON(sc); TSL_POISON(part); TSL_POISON(red);
     const int tid = threadIdx.x;
-    const int c = blockIdx.x % a.NCH;
-    const long bg = blockIdx.x / a.NCH;
+    const int c = blockIdx.x / (a.B * a.G);
+    const long bg = blockIdx.x % (a.B * a.G);
     const int g = bg % a.G, b = bg / a.G;
     const int n = tokens_of(a, b);
-    const int nact = max(1, (int)(((long)n + a.CT - 1) / a.CT));  // (at most NCH)
-    if (c >= nact) return;
+    if (n <= c * a.CT) {
+        if (c == 0)  // an empty sequence: 0 / 0
+            for (int i = tid; i < QPG * D; i += 256) a.O[((long)b * a.H + g * QPG) * D + i] = 0x7e00;
+        return;
+    }
     const int t_lo = c * a.CT, t_hi = min(n - t_lo, a.CT) + t_lo;
     for (int i = tid; i < QPG * D; i += 256) qs[i / D][i % D] = h2f(a.Q[((long)b * a.H + g * QPG) * D + i]);
     if (tid < QPG) mrun[tid] = -INFINITY, lrun[tid] = 0.0f, lowsum[tid] = 0.0f;
@@ -158,51 +162,369 @@ __global__ __launch_bounds__(256) void decode_q4_any(Q4Args a) {
     }
 }
 
-// Joins a (sequence, query head)'s chunks in order; a wavefront each.
-template <int D>
-__global__ __launch_bounds__(64) void decode_q4_join(Q4Args a, int qpg) {
-    const int h = blockIdx.x % a.H, g = h / qpg, i = h % qpg;
-    const long b = blockIdx.x / a.H;
-    const int nact = max(1, (int)(((long)tokens_of(a, b) + a.CT - 1) / a.CT));
-    const float* p = a.part + ((b * a.G + g) * a.NCH * qpg + i) * (2L + D);
-    const long next = (long)qpg * (2 + D);
-    float m = -INFINITY;
-    for (int c = 0; c < nact; c++) m = fmaxf(m, p[c * next]);
-    for (int d = threadIdx.x; d < D; d += 64) {
-        float l = 0.0f, v = 0.0f;
-        for (int c = 0; c < nact; c++) {
-            const float f = __builtin_amdgcn_exp2f(p[c * next] - m);
-            l += p[c * next + 1] * f;
-            v += p[c * next + 2 + d] * f;
+// ---------------------------------------------------------------- the matrix-core form
+// D = 32, 64 or 128. A workgroup of NW wavefronts has one (sequence, kv head, chunk of at most
+// CHUNK_MAX tokens); wavefront w takes the 64-token tiles w, w + NW, .. of the chunk, the next
+// tile's loads in flight. All of a tile goes from memory into registers in the operands' own shapes:
+//
+//   S^T = K Q^T, four tiles of 16 tokens x 16 query heads (v_mfma_f32_16x16x32_f16): row i of tile a is
+//   token 4 a + i % 4 of block i / 4 (a tile of 64 tokens is 4 blocks of 16), so that lane (head, g) ends with
+//   the 16 tokens of block g in order; its 16 bytes of V's layout are those tokens of a channel pair:
+//   O^T += V^T P^T, 16 channels x 16 heads a tile, channels of one parity, tokens 8 u .. 8 u + 7 of every block a step.
+//
+// A code needs no conversion: as the low bits of an f16 it is the subnormal n 2^-24, which the matrix cores
+// multiply exactly, in the next four bits n 2^-20. One shift and four ands so make 8 operand values of a word
+// (pairs of bytes 0, 2 and 1, 3, low and high nibbles): v_mfma sees n 2^-24 and 16 n 2^-24, and the
+// 16 is taken out of q's odd channels (q is scaled by a power of two into f16's
+// middle) and of the odd output channels at the end. step and low enter in f32: u = step (q . n) + low sum(q);
+// p step is split into two f16, so a probability keeps 22 bits.
+//
+// Bound by memory for long caches, and by VALU not far below (about 25 operations a score of 16, mostly
+// lanes of unused heads where H / G < 16).
+constexpr int TILE = 64;
+constexpr int CHUNK_MAX = 1024;  // tokens: a table entry a lane at 16 tokens a page
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x4 u32x4u __attribute__((aligned(2)));
+
+template <int W>
+struct Words {  // a lane's W words of a row
+    uint32_t w[W];
+    TSL_DEV void load(const uint8_t* p) {
+        if constexpr (W == 4) {
+            const u32x4 v = *reinterpret_cast<const u32x4*>(p);
+            w[0] = v[0], w[1] = v[1], w[2] = v[2], w[3] = v[3];
+        } else if constexpr (W == 2) {
+            const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+            w[0] = v[0], w[1] = v[1];
+        } else {
+            w[0] = *reinterpret_cast<const uint32_t*>(p);
         }
-        a.O[(b * a.H + h) * D + d] = f2h(v / l);
+    }
+};
+
+// f16 pairs of a word's codes: low nibbles of bytes (0, 2), (1, 3), then high nibbles.
+TSL_DEV void nibbles(uint32_t w, uint32_t (&lo)[2], uint32_t (&hi)[2]) {
+    const uint32_t v = w >> 8;
+    lo[0] = w & 0x000f000fu, lo[1] = v & 0x000f000fu;
+    hi[0] = w & 0x00f000f0u, hi[1] = v & 0x00f000f0u;
+}
+TSL_DEV half8 half8_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __builtin_bit_cast(half8, u32x4{a, b, c, d}); }
+
+TSL_DEV float lo_h(uint32_t w) { return (float)as_half2(w)[0]; }
+TSL_DEV float hi_h(uint32_t w) { return (float)as_half2(w)[1]; }
+
+// The value of the lane that holds token T in this lane's row of 16 (row_newbcast).
+TSL_DEV uint32_t of_token(uint32_t x, int t) {
+    switch (t) {
+#define Q4_TOKEN(T) \
+    case T: return __builtin_amdgcn_mov_dpp((int)x, 0x150 + T, 0xf, 0xf, false);
+        Q4_TOKEN(0) Q4_TOKEN(1) Q4_TOKEN(2) Q4_TOKEN(3) Q4_TOKEN(4) Q4_TOKEN(5) Q4_TOKEN(6) Q4_TOKEN(7)
+        Q4_TOKEN(8) Q4_TOKEN(9) Q4_TOKEN(10) Q4_TOKEN(11) Q4_TOKEN(12) Q4_TOKEN(13) Q4_TOKEN(14)
+#undef Q4_TOKEN
+        default: return __builtin_amdgcn_mov_dpp((int)x, 0x15f, 0xf, 0xf, false);
     }
 }
 
-// Tokens a chunk: 256 at least, and about 2048 workgroups at the table's full length.
+template <int D>
+struct Q4Tile {
+    Words<D / 32> k[4];  // tile i: token 4 i + l % 4 of block (l % 16) / 4, bytes (D / 8) (l / 16) ..
+    Words<4> v[D / 32];  // channel pair 16 j + l % 16, the 16 tokens of block l / 16
+    uint32_t ks, vs;     // (low, step) of token l % 16 of block l / 16
+};
+
+template <int D, int QPG, int NW>
+__global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q4_mfma(Q4Args a) {
+    constexpr int KW = D / 32, NT = D / 16, CB = D / 8;  // words of a K row a lane; channel tiles; their bytes
+    constexpr float GROW = 2.0f;                        // p <= 2^GROW: p step stays in f16
+    constexpr int COLS = D + 2;
+    __shared__ float red[NW][QPG][COLS];
+    TSL_POISON(red);
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // Chunk after chunk: workgroups go round the XCDs, and with a sequence's chunks side by side some XCDs had
+    // the first ones, which all sequences have, and others the last (64 of 128-4096 tokens 57.7 us).
+    const int c = blockIdx.x / (a.B * a.G), bg = blockIdx.x % (a.B * a.G);
+    const int g = bg % a.G, b = bg / a.G;
+    // The length, the chunk's table entries (one a lane; t_in: where in its first page it begins) and q in
+    // one round trip: none of these loads depends on another.
+    const int t_lo = c * a.CT, t_in = t_lo & (a.P - 1);
+    const int held = (t_in + min(a.CT, a.MP * a.P - t_lo) + a.P - 1) >> a.pshift;
+    const int tab = lane < held ? a.table[(long)b * a.MP + (t_lo >> a.pshift) + lane] : 0;
+    float qs[2 * CB];
+#pragma unroll
+    for (int i = 0; i < 2 * CB; i++) qs[i] = 0.0f;
+    if (l16 < QPG) {  // head l16's channels 2 CB g4 .. 2 CB g4 + 2 CB - 1
+        const u16* qp = a.Q + ((long)b * a.H + g * QPG + l16) * D + 2 * CB * g4;
+#pragma unroll
+        for (int i = 0; i < CB / 4; i++) {
+            const u32x4 t = *reinterpret_cast<const u32x4u*>(qp + 8 * i);
+#pragma unroll
+            for (int e = 0; e < 8; e++) qs[8 * i + e] = h2f((u16)(t[e >> 1] >> (16 * (e & 1))));
+        }
+    }
+    const int n = tokens_of(a, b);
+    const int len = min(n - t_lo, a.CT);  // this chunk's tokens
+    if (len <= 0) {
+        if (c == 0)  // an empty sequence: 0 / 0
+            for (int i = threadIdx.x; i < QPG * D; i += 64 * NW) a.O[((long)b * a.H + g * QPG) * D + i] = 0x7e00;
+        return;
+    }
+    const int entries = (t_in + len + a.P - 1) >> a.pshift;
+
+    // Word w's eight channels are a step's operand.
+    float qmax = 0.0f, qsum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2 * CB; i++) {
+        qmax = fmaxf(qmax, __builtin_fabsf(qs[i]));
+        qsum += qs[i];
+    }
+    qmax = fmaxf(qmax, xor16(qmax));
+    qmax = fmaxf(qmax, xor32(qmax));
+    qsum += xor16(qsum);
+    qsum += xor32(qsum);
+    // 2^eq brings the largest magnitude into [2^10, 2^11); an infinity or zeros stay.
+    const int eq = qmax > 0.0f && qmax <= 65504.0f ? 10 - __builtin_amdgcn_frexp_expf(qmax) + 1 : 0;
+    const float up = __builtin_ldexpf(a.c2 < 0.0f ? -1.0f : 1.0f, eq);  // (a negative scale: q turned over)
+    half8 qop[KW];
+#pragma unroll
+    for (int w = 0; w < KW; w++) {
+        // Nibble e of a word is channel 8 w + e; its operand order: 0 4 2 6 (low) 1 5 3 7 (high, / 16).
+        constexpr int at[8] = {0, 4, 2, 6, 1, 5, 3, 7};
+#pragma unroll
+        for (int e = 0; e < 8; e++) qop[w][e] = (half_t)(qs[8 * w + at[e]] * (e < 4 ? up : up * 0.0625f));
+    }
+    const float cs = fmaxf(__builtin_ldexpf(__builtin_fabsf(a.c2), 24 - eq), 1e-37f);  // of u's units (a scale of 0: nearly)
+    const float qz = __builtin_ldexpf(qsum, eq - 24) * (a.c2 < 0.0f ? -1.0f : 1.0f);
+
+    const int ntiles = (len + TILE - 1) / TILE;
+    const int kb = (l16 >> 2), kt = l16 & 3;  // this lane's block and token of K's tiles
+    const int blocks = a.P >> 4;              // blocks of 16 tokens a page
+    // The page of the chunk's p-th block of 16 tokens (-1: outside the pool or past the chunk), and
+    // where the block is in the pool (page 0's for none: its bytes are read, its pairs are not used).
+    auto page_at = [&](int p) {
+        const int e = (t_in + 16 * p) >> a.pshift;
+        const int page = __builtin_amdgcn_ds_bpermute(4 * min(e, 63), tab);
+        return e < entries && page < a.NP ? page : -1;
+    };
+    auto block_at = [&](int p) { return ((long)max(page_at(p), 0) * a.G + g) * blocks + (((t_in >> 4) + p) & (blocks - 1)); };
+    // Loads are issued whether or not the tile exists (past the chunk the last one's again, from the caches): behind
+    // a branch the compiler could not count on them and waited for all.
+    auto load = [&](int tile, Q4Tile<D>& x) {
+        tile = min(tile, ntiles - 1);
+        const long bk = block_at(4 * tile + kb), bv = block_at(4 * tile + g4);
+        const uint8_t* kp = a.Kc + bk * (8 * D) + kt * (D / 2) + CB * g4;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x.k[i].load(kp + i * (2 * D));
+        x.ks = reinterpret_cast<const uint32_t*>(a.Ks)[bv * 16 + l16];
+        x.vs = reinterpret_cast<const uint32_t*>(a.Vs)[bv * 16 + l16];
+        const uint8_t* vp = a.Vc + bv * (8 * D) + l16 * 16;
+#pragma unroll
+        for (int j = 0; j < KW; j++) x.v[j].load(vp + j * 256);
+    };
+
+    float m = -INFINITY, l = 0.0f, low = 0.0f;  // running maximum of u; sums of p and p low (this lane's tokens)
+    float4v acc[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++) acc[i] = float4v{};
+    auto step = [&](int tile, Q4Tile<D>& x) {
+        // Tokens past the end, and pages outside the pool: pairs of zeros (what the
+        // cache holds there is not looked at; a spoilt pair would spoil 0 x it).
+        const int left = len - tile * TILE - 16 * g4;  // of this lane's block
+        const bool tail = __builtin_amdgcn_ballot_w64(left < 16) != 0;
+        if (l16 >= left || page_at(4 * tile + g4) < 0) x.ks = x.vs = 0;
+        float u[16];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            float4v s = float4v{};
+#pragma unroll
+            for (int w = 0; w < KW; w++) {
+                uint32_t nl[2], nh[2];
+                nibbles(x.k[t].w[w], nl, nh);
+                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(half8_of(nl[0], nl[1], nh[0], nh[1]), qop[w], s, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const uint32_t pair = of_token(x.ks, 4 * t + r);
+                u[4 * t + r] = __builtin_fmaf(hi_h(pair), s[r], lo_h(pair) * qz);
+            }
+        }
+        if (tail) {
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (i >= left) u[i] = -INFINITY;
+        }
+        float mx = u[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) mx = fmaxf(mx, u[i]);
+        if (__builtin_amdgcn_ballot_w64((mx - m) * cs > GROW)) {  // some head's maximum moves: all of its lanes'
+            mx = fmaxf(mx, xor16(mx));
+            mx = fmaxf(fmaxf(mx, xor32(mx)), m);
+            const float f = m == mx ? 1.0f : __builtin_amdgcn_exp2f((m - mx) * cs);
+            m = mx;
+            l *= f;
+            low *= f;
+#pragma unroll
+            for (int i = 0; i < NT; i++) acc[i] *= f;
+        }
+        const float off = -m * cs;
+        uint32_t ph[8], pl[8];  // p step in two f16, in V's token order: 0 2, 1 3 of every four
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            half_t h[4], e[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(u[4 * t + r], cs, off));
+                const uint32_t pair = of_token(x.vs, 4 * t + r);
+                l += p;
+                low = __builtin_fmaf(p, lo_h(pair), low);
+                const float w = p * hi_h(pair);
+                h[r] = (half_t)w;
+                e[r] = (half_t)(w - (float)h[r]);
+            }
+            ph[2 * t] = __builtin_bit_cast(uint32_t, half2v{h[0], h[2]});
+            ph[2 * t + 1] = __builtin_bit_cast(uint32_t, half2v{h[1], h[3]});
+            pl[2 * t] = __builtin_bit_cast(uint32_t, half2v{e[0], e[2]});
+            pl[2 * t + 1] = __builtin_bit_cast(uint32_t, half2v{e[1], e[3]});
+        }
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const half8 hp = half8_of(ph[4 * s], ph[4 * s + 1], ph[4 * s + 2], ph[4 * s + 3]);
+            const half8 ep = half8_of(pl[4 * s], pl[4 * s + 1], pl[4 * s + 2], pl[4 * s + 3]);
+#pragma unroll
+            for (int j = 0; j < D / 32; j++) {
+                uint32_t l0[2], h0[2], l1[2], h1[2];
+                nibbles(x.v[j].w[2 * s], l0, h0);
+                nibbles(x.v[j].w[2 * s + 1], l1, h1);
+                const half8 even = half8_of(l0[0], l0[1], l1[0], l1[1]), odd = half8_of(h0[0], h0[1], h1[0], h1[1]);
+                acc[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, hp, acc[2 * j], 0, 0, 0);
+                acc[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, hp, acc[2 * j + 1], 0, 0, 0);
+                acc[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, ep, acc[2 * j], 0, 0, 0);
+                acc[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, ep, acc[2 * j + 1], 0, 0, 0);
+            }
+        }
+    };
+    Q4Tile<D> x, y;
+    load(wave, x);
+    for (int t = wave; t < ntiles; t += 2 * NW) {
+        load(t + NW, y);
+        step(t, x);
+        if (t + NW >= ntiles) break;
+        load(t + 2 * NW, x);
+        step(t + NW, y);
+    }
+    // The wavefronts' states, joined in order: the maximum (log2 units), sums, outputs.
+    l += xor16(l);
+    l += xor32(l);
+    low += xor16(low);
+    low += xor32(low);
+    if (l16 < QPG) {
+#pragma unroll
+        for (int j = 0; j < D / 32; j++)
+#pragma unroll
+            for (int e = 0; e < 2; e++)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    red[wave][l16][2 * (16 * j + 4 * g4 + r) + e] =
+                        __builtin_fmaf(acc[2 * j + e][r], e ? 0x1p20f : 0x1p24f, low);
+        if (g4 == 0) red[wave][l16][D] = m * cs, red[wave][l16][D + 1] = l;
+    }
+    __syncthreads();
+    const int active = min(NW, ntiles);
+    for (int i = threadIdx.x; i < QPG * D; i += 64 * NW) {
+        const int h = i / D, d = i % D;
+        float top = red[0][h][D];
+        for (int w = 1; w < active; w++) top = fmaxf(top, red[w][h][D]);
+        float sum = 0.0f, v = 0.0f;
+        for (int w = 0; w < active; w++) {
+            const float f = __builtin_amdgcn_exp2f(red[w][h][D] - top);
+            sum = __builtin_fmaf(red[w][h][D + 1], f, sum);
+            v = __builtin_fmaf(red[w][h][d], f, v);
+        }
+        if (a.NCH == 1) {
+            a.O[((long)b * a.H + g * QPG + h) * D + d] = f2h(v / sum);
+        } else {
+            float* p = a.part + (((long)bg * a.NCH + c) * QPG + h) * (2 + D);
+            if (d == 0) p[0] = top, p[1] = sum;
+            p[2 + d] = v;
+        }
+    }
+}
+
+// Joins a (sequence, query head)'s chunks in order. Four wavefronts take every fourth chunk.
+template <int D>
+__global__ __launch_bounds__(256) void decode_q4_join(Q4Args a, int qpg) {
+    __shared__ float red[4][D + 2];
+    TSL_POISON(red);
+    const int h = blockIdx.x % a.H, g = h / qpg, i = h % qpg;
+    const long b = blockIdx.x / a.H;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int nact = (int)(((long)tokens_of(a, b) + a.CT - 1) / a.CT);
+    if (nact == 0) return;  // (an empty sequence: written already)
+    const float* p = a.part + ((b * a.G + g) * a.NCH * qpg + i) * (2L + D);
+    const long next = (long)qpg * (2 + D);
+    float m = -INFINITY, l = 0.0f, v[(D + 63) / 64];
+    for (int c = lane; c < nact; c += 64) m = fmaxf(m, p[c * next]);
+    m = wave_max(m);
+#pragma unroll
+    for (int k = 0; k < (D + 63) / 64; k++) v[k] = 0.0f;
+#pragma unroll 4
+    for (int c = wave; c < nact; c += 4) {
+        const float f = __builtin_amdgcn_exp2f(p[c * next] - m);
+        l = __builtin_fmaf(p[c * next + 1], f, l);
+#pragma unroll
+        for (int k = 0; k < (D + 63) / 64; k++)
+            if (D >= 64 || lane < D) v[k] = __builtin_fmaf(p[c * next + 2 + 64 * k + lane], f, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < (D + 63) / 64; k++)
+        if (D >= 64 || lane < D) red[wave][64 * k + lane] = v[k];
+    if (lane == 0) red[wave][D] = l;
+    __syncthreads();
+    if (threadIdx.x < D) {
+        const int d = threadIdx.x;
+        const float sum = (red[0][D] + red[1][D]) + (red[2][D] + red[3][D]);
+        a.O[(b * a.H + h) * D + d] = f2h(((red[0][d] + red[1][d]) + (red[2][d] + red[3][d])) / sum);
+    }
+}
+
+// Tokens a chunk. Tables of at most CHUNK_MAX tokens are one chunk (no second launch); longer
+// ones are cut into 256 to CHUNK_MAX tokens, about 8 workgroups a CU at the table's full length, which even out
+// lengths that differ.
 int chunk_tokens(const TslKernel& k) {
     const int64_t bg = std::max<int64_t>(1, k.dim("B") * k.dim("G")), most = k.dim("MP") * k.dim("P");
-    return (int)std::min<int64_t>(std::max<int64_t>(256, (most * bg / 2048 + 255) / 256 * 256), 1 << 24);
+    if (most <= CHUNK_MAX) return CHUNK_MAX;
+    return (int)std::min<int64_t>(std::max<int64_t>(256, (most * bg / (8 * num_cus()) + 255) / 256 * 256), CHUNK_MAX);
 }
 int nchunks(const TslKernel& k) {
     const int64_t most = k.dim("MP") * k.dim("P"), ct = chunk_tokens(k);
     return (int)std::max<int64_t>(1, (most + ct - 1) / ct);
 }
 
-template <int D>
-int run_q4(const Q4Args& a, int qpg, hipStream_t s) {
-    const unsigned grid = (unsigned)((long)a.B * a.G * a.NCH);
-    switch (qpg) {
-        case 1: hipLaunchKernelGGL((decode_q4_any<D, 1>), dim3(grid), dim3(256), 0, s, a); break;
-        case 2: hipLaunchKernelGGL((decode_q4_any<D, 2>), dim3(grid), dim3(256), 0, s, a); break;
-        case 4: hipLaunchKernelGGL((decode_q4_any<D, 4>), dim3(grid), dim3(256), 0, s, a); break;
-        case 8: hipLaunchKernelGGL((decode_q4_any<D, 8>), dim3(grid), dim3(256), 0, s, a); break;
-        default: hipLaunchKernelGGL((decode_q4_any<D, 16>), dim3(grid), dim3(256), 0, s, a); break;
+template <int D, int QPG>
+int run_q4(const Q4Args& a, hipStream_t s) {
+    const dim3 grid((unsigned)((long)a.B * a.G * a.NCH));
+    if constexpr (D == 16) {
+        hipLaunchKernelGGL((decode_q4_any<D, QPG>), grid, dim3(256), 0, s, a);
+    } else {
+        if (a.NCH == 1) hipLaunchKernelGGL((decode_q4_mfma<D, QPG, 8>), grid, dim3(512), 0, s, a);
+        else hipLaunchKernelGGL((decode_q4_mfma<D, QPG, 4>), grid, dim3(256), 0, s, a);
     }
     int r = TSL_LAUNCHED("quant decode_attention");
     if (r || a.NCH == 1) return r;
-    hipLaunchKernelGGL(decode_q4_join<D>, dim3((unsigned)((long)a.B * a.H)), dim3(64), 0, s, a, qpg);
+    hipLaunchKernelGGL(decode_q4_join<D>, dim3((unsigned)((long)a.B * a.H)), dim3(256), 0, s, a, QPG);
     return TSL_LAUNCHED("quant decode_attention join");
+}
+
+template <int D>
+int run_q4_d(const Q4Args& a, hipStream_t s) {
+    switch (a.H / a.G) {
+        case 1: return run_q4<D, 1>(a, s);
+        case 2: return run_q4<D, 2>(a, s);
+        case 4: return run_q4<D, 4>(a, s);
+        case 8: return run_q4<D, 8>(a, s);
+        default: return run_q4<D, 16>(a, s);
+    }
 }
 
 }  // namespace
@@ -214,6 +536,7 @@ int check_decode_q4(TslKernel& k) {
     const int64_t qpg = H / G;
     if (qpg != 1 && qpg != 2 && qpg != 4 && qpg != 8 && qpg != 16)
         return tsl_fail(-2, "quant/decode_attention: H / G must be 1, 2, 4, 8 or 16");
+    if (k.dim("NP") == 0) return tsl_fail(-2, "quant/decode_attention: a pool of no pages");
     if (MP > INT_MAX / k.dim("P") || B * H > (1 << 24) || B * G * nchunks(k) > (1 << 24))
         return tsl_fail(-2, "quant/decode_attention: at most 2^31 - 1 tokens a table and 2^24 (sequence, head, chunk)s");
     return 0;
@@ -240,14 +563,13 @@ int launch_decode_q4(TslKernel& k, const uint64_t* args, hipStream_t s) {
     a.O = P<u16>(args[7]);
     a.c2 = arg_f32(args[8]) * LOG2E;
     a.B = k.dim("B"), a.H = k.dim("H"), a.G = k.dim("G"), a.NP = k.dim("NP"), a.P = k.dim("P"), a.MP = k.dim("MP");
-    a.NCH = nchunks(k), a.CT = chunk_tokens(k);
+    a.NCH = nchunks(k), a.CT = chunk_tokens(k), a.pshift = __builtin_ctz((unsigned)a.P);
     a.part = reinterpret_cast<float*>(k.scratch);
     if (a.B == 0) return 0;
-    const int qpg = a.H / a.G;
     switch (k.dim("D")) {
-        case 16: return run_q4<16>(a, qpg, s);
-        case 32: return run_q4<32>(a, qpg, s);
-        case 64: return run_q4<64>(a, qpg, s);
-        default: return run_q4<128>(a, qpg, s);
+        case 16: return run_q4_d<16>(a, s);
+        case 32: return run_q4_d<32>(a, s);
+        case 64: return run_q4_d<64>(a, s);
+        default: return run_q4_d<128>(a, s);
     }
 }

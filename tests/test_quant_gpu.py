@@ -309,7 +309,9 @@ ATTENTION = [(1, 4, 2, 16, 16, [1]), (2, 8, 4, 32, 16, [15, 17]), (3, 32, 4, 64,
              (2, 32, 8, 128, 16, [63, 64]), (4, 16, 16, 64, 32, [65, 0, 31, 200]), (1, 16, 1, 128, 16, [1000]),
              (5, 8, 2, 64, 64, [5, 64, 129, 700, 2]), (1, 32, 4, 64, 16, [5000]), (2, 16, 2, 128, 32, [2111, 3]),
              (7, 4, 4, 128, 16, [1, 2, 3, 4, 255, 256, 257]), (2, 16, 1, 16, 16, [300, 40]), (1, 2, 1, 32, 128, [1500]),
-             (40, 8, 8, 128, 16, list(range(1, 400, 10))), (1, 8, 1, 64, 16, [4097])]
+             (40, 8, 8, 128, 16, list(range(1, 400, 10))), (1, 8, 1, 64, 16, [4097]), (3, 4, 2, 16, 16, [1500, 0, 300]),
+             (2, 4, 1, 128, 512, [2000, 700]), (2, 8, 4, 64, 2048, [2049, 5000]), (1, 8, 8, 32, 256, [1025]),
+             (300, 4, 4, 64, 16, [1100] + [5, 0, 64] * 99 + [1023, 33]), (2, 32, 2, 64, 1024, [0, 3000])]
 
 
 @pytest.mark.parametrize("b,h,g,d,p,lens", ATTENTION)
