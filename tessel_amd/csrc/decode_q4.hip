@@ -31,6 +31,7 @@ struct Q4Args {
     int B, H, G, NP, P, MP, NCH;
     int CT;       // tokens per chunk (a multiple of 256)
     int pshift;   // log2(P)
+    bool wide;    // one chunk a sequence, 8 wavefronts
     float c2;     // scale log2(e)
 };
 
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(256) void decode_q4_any(Q4Args a) {
 // Bound by memory for long caches, and by VALU not far below (about 25 operations a score of 16, mostly
 // lanes of unused heads where H / G < 16).
 constexpr int TILE = 64;
-constexpr int CHUNK_MAX = 1024;  // tokens: a table entry a lane at 16 tokens a page
+constexpr int CHUNK_MAX = 4096;  // tokens of a chunk, at most (their table entries are held in LDS)
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x4 u32x4u __attribute__((aligned(2)));
@@ -226,31 +227,99 @@ TSL_DEV uint32_t of_token(uint32_t x, int t) {
     }
 }
 
-template <int D>
+// (low, step) pairs of a lane's tokens: CF = 1 holds one token's a lane and
+// hands them round, else a lane loads its own 16 / CF.
+template <int CF>
+struct Pairs {
+    Words<4> w[4 / CF];
+    TSL_DEV void load(const u16* p, long block, int l16) {
+        const uint8_t* q = reinterpret_cast<const uint8_t*>(p + block * 32) + (l16 / (16 / CF)) * (64 / CF);
+#pragma unroll
+        for (int i = 0; i < 4 / CF; i++) w[i].load(q + 16 * i);
+    }
+    TSL_DEV uint32_t get(int i) const { return w[i / 4].w[i % 4]; }
+    TSL_DEV void drop(int first, int left, bool all) {  // tokens first + .. at left and past it, or all of them
+#pragma unroll
+        for (int i = 0; i < 16 / CF; i++)
+            if (all || first + i >= left) w[i / 4].w[i % 4] = 0;
+    }
+};
+template <>
+struct Pairs<1> {
+    uint32_t w;
+    TSL_DEV void load(const u16* p, long block, int l16) { w = reinterpret_cast<const uint32_t*>(p)[block * 16 + l16]; }
+    TSL_DEV uint32_t get(int i) const { return of_token(w, i); }
+    TSL_DEV void drop(int, int left, bool all) {
+        if (all || (int)(threadIdx.x & 15) >= left) w = 0;
+    }
+};
+
+template <int D, int CF>
 struct Q4Tile {
     Words<D / 32> k[4];  // tile i: token 4 i + l % 4 of block (l % 16) / 4, bytes (D / 8) (l / 16) ..
     Words<4> v[D / 32];  // channel pair 16 j + l % 16, the 16 tokens of block l / 16
-    uint32_t ks, vs;     // (low, step) of token l % 16 of block l / 16
+    Pairs<CF> ks, vs;    // of this lane's tokens of block l / 16
 };
+
+// Lanes 16 / CF j .. of every row of 16 take part j's value from the row's first lanes (pack), and back (part).
+template <int CF>
+TSL_DEV float pack_lanes(const float (&s)[CF]) {
+    int v = __builtin_bit_cast(int, s[0]);
+    if constexpr (CF == 2) {
+        v = __builtin_amdgcn_update_dpp(v, __builtin_bit_cast(int, s[1]), 0x118, 0xf, 0xc, false);  // row_shr:8
+    } else if constexpr (CF == 4) {
+        v = __builtin_amdgcn_update_dpp(v, __builtin_bit_cast(int, s[1]), 0x114, 0xf, 0x2, false);  // row_shr:4, 8, 12
+        v = __builtin_amdgcn_update_dpp(v, __builtin_bit_cast(int, s[2]), 0x118, 0xf, 0x4, false);
+        v = __builtin_amdgcn_update_dpp(v, __builtin_bit_cast(int, s[3]), 0x11c, 0xf, 0x8, false);
+    }
+    return __builtin_bit_cast(float, v);
+}
+template <int CF>
+TSL_DEV uint32_t part_lanes(uint32_t x, int j) {
+    if (j == 0) return x;
+    if constexpr (CF == 2) return __builtin_amdgcn_mov_dpp((int)x, 0x108, 0xf, 0xf, true);  // row_shl:8
+    if (j == 1) return __builtin_amdgcn_mov_dpp((int)x, 0x104, 0xf, 0xf, true);
+    if (j == 2) return __builtin_amdgcn_mov_dpp((int)x, 0x108, 0xf, 0xf, true);
+    return __builtin_amdgcn_mov_dpp((int)x, 0x10c, 0xf, 0xf, true);
+}
+// Over the lanes that share a head: those 16 / CF apart in a row, and the four rows.
+template <int CF>
+TSL_DEV float head_max(float x) {
+    if constexpr (CF >= 2) x = fmaxf(x, __shfl_xor(x, 8));
+    if constexpr (CF >= 4) x = fmaxf(x, __shfl_xor(x, 4));
+    x = fmaxf(x, xor16(x));
+    return fmaxf(x, xor32(x));
+}
+template <int CF>
+TSL_DEV float head_sum(float x) {
+    if constexpr (CF >= 2) x += __shfl_xor(x, 8);
+    if constexpr (CF >= 4) x += __shfl_xor(x, 4);
+    x += xor16(x);
+    return x + xor32(x);
+}
 
 template <int D, int QPG, int NW>
 __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q4_mfma(Q4Args a) {
     constexpr int KW = D / 32, NT = D / 16, CB = D / 8;  // words of a K row a lane; channel tiles; their bytes
     constexpr float GROW = 2.0f;                        // p <= 2^GROW: p step stays in f16
+    // Few query heads leave most of the 16 columns empty: the scores of four (two)
+    // of a lane's tiles are packed onto the row's lanes, 16 / CF a lane, for the softmax.
+    constexpr int CF = QPG <= 4 ? 4 : QPG == 8 ? 2 : 1, TPL = 16 / CF;
     constexpr int COLS = D + 2;
     __shared__ float red[NW][QPG][COLS];
-    TSL_POISON(red);
+    __shared__ int tab[CHUNK_MAX / 16];
+    TSL_POISON(red); TSL_POISON(tab);
     const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Chunk after chunk: workgroups go round the XCDs, and with a sequence's chunks side by side some XCDs had
     // the first ones, which all sequences have, and others the last (64 of 128-4096 tokens 57.7 us).
     const int c = blockIdx.x / (a.B * a.G), bg = blockIdx.x % (a.B * a.G);
     const int g = bg % a.G, b = bg / a.G;
-    // The length, the chunk's table entries (one a lane; t_in: where in its first page it begins) and q in
+    // The length, the chunk's table entries (t_in: where in its first page it begins) and q in
     // one round trip: none of these loads depends on another.
     const int t_lo = c * a.CT, t_in = t_lo & (a.P - 1);
     const int held = (t_in + min(a.CT, a.MP * a.P - t_lo) + a.P - 1) >> a.pshift;
-    const int tab = lane < held ? a.table[(long)b * a.MP + (t_lo >> a.pshift) + lane] : 0;
+    for (int e = threadIdx.x; e < held; e += 64 * NW) tab[e] = a.table[(long)b * a.MP + (t_lo >> a.pshift) + e];
     float qs[2 * CB];
 #pragma unroll
     for (int i = 0; i < 2 * CB; i++) qs[i] = 0.0f;
@@ -271,6 +340,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
         return;
     }
     const int entries = (t_in + len + a.P - 1) >> a.pshift;
+    __syncthreads();  // (tab)
 
     // Word w's eight channels are a step's operand.
     float qmax = 0.0f, qsum = 0.0f;
@@ -294,8 +364,10 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
 #pragma unroll
         for (int e = 0; e < 8; e++) qop[w][e] = (half_t)(qs[8 * w + at[e]] * (e < 4 ? up : up * 0.0625f));
     }
-    const float cs = fmaxf(__builtin_ldexpf(__builtin_fabsf(a.c2), 24 - eq), 1e-37f);  // of u's units (a scale of 0: nearly)
-    const float qz = __builtin_ldexpf(qsum, eq - 24) * (a.c2 < 0.0f ? -1.0f : 1.0f);
+    // Of the head whose scores this lane takes (l16 % TPL): u's units (a scale of 0: nearly), and low's factor.
+    const int head = (lane & 48) + l16 % TPL;
+    const float cs = __shfl(fmaxf(__builtin_ldexpf(__builtin_fabsf(a.c2), 24 - eq), 1e-37f), head);
+    const float qz = __shfl(__builtin_ldexpf(qsum, eq - 24) * (a.c2 < 0.0f ? -1.0f : 1.0f), head);
 
     const int ntiles = (len + TILE - 1) / TILE;
     const int kb = (l16 >> 2), kt = l16 & 3;  // this lane's block and token of K's tiles
@@ -304,20 +376,20 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
     // where the block is in the pool (page 0's for none: its bytes are read, its pairs are not used).
     auto page_at = [&](int p) {
         const int e = (t_in + 16 * p) >> a.pshift;
-        const int page = __builtin_amdgcn_ds_bpermute(4 * min(e, 63), tab);
+        const int page = tab[min(e, entries - 1)];
         return e < entries && page < a.NP ? page : -1;
     };
     auto block_at = [&](int p) { return ((long)max(page_at(p), 0) * a.G + g) * blocks + (((t_in >> 4) + p) & (blocks - 1)); };
     // Loads are issued whether or not the tile exists (past the chunk the last one's again, from the caches): behind
     // a branch the compiler could not count on them and waited for all.
-    auto load = [&](int tile, Q4Tile<D>& x) {
+    auto load = [&](int tile, Q4Tile<D, CF>& x) {
         tile = min(tile, ntiles - 1);
         const long bk = block_at(4 * tile + kb), bv = block_at(4 * tile + g4);
         const uint8_t* kp = a.Kc + bk * (8 * D) + kt * (D / 2) + CB * g4;
 #pragma unroll
         for (int i = 0; i < 4; i++) x.k[i].load(kp + i * (2 * D));
-        x.ks = reinterpret_cast<const uint32_t*>(a.Ks)[bv * 16 + l16];
-        x.vs = reinterpret_cast<const uint32_t*>(a.Vs)[bv * 16 + l16];
+        x.ks.load(a.Ks, bv, l16);
+        x.vs.load(a.Vs, bv, l16);
         const uint8_t* vp = a.Vc + bv * (8 * D) + l16 * 16;
 #pragma unroll
         for (int j = 0; j < KW; j++) x.v[j].load(vp + j * 256);
@@ -327,39 +399,46 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
     float4v acc[NT];
 #pragma unroll
     for (int i = 0; i < NT; i++) acc[i] = float4v{};
-    auto step = [&](int tile, Q4Tile<D>& x) {
+    auto step = [&](int tile, Q4Tile<D, CF>& x) {
         // Tokens past the end, and pages outside the pool: pairs of zeros (what the
         // cache holds there is not looked at; a spoilt pair would spoil 0 x it).
         const int left = len - tile * TILE - 16 * g4;  // of this lane's block
-        const bool tail = __builtin_amdgcn_ballot_w64(left < 16) != 0;
-        if (l16 >= left || page_at(4 * tile + g4) < 0) x.ks = x.vs = 0;
-        float u[16];
+        const int first = (l16 / TPL) * (CF == 1 ? 0 : TPL);  // this lane's tokens of it: first ..
+        const bool none = page_at(4 * tile + g4) < 0, tail = __builtin_amdgcn_ballot_w64(left < 16) != 0;
+        if (tail || __builtin_amdgcn_ballot_w64(none)) {
+            x.ks.drop(first, left, none);
+            x.vs.drop(first, left, none);
+        }
+        float4v s[4];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            float4v s = float4v{};
+            s[t] = float4v{};
 #pragma unroll
             for (int w = 0; w < KW; w++) {
                 uint32_t nl[2], nh[2];
                 nibbles(x.k[t].w[w], nl, nh);
-                s = __builtin_amdgcn_mfma_f32_16x16x32_f16(half8_of(nl[0], nl[1], nh[0], nh[1]), qop[w], s, 0, 0, 0);
+                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(half8_of(nl[0], nl[1], nh[0], nh[1]), qop[w], s[t], 0, 0, 0);
             }
+        }
+        float u[TPL];  // token first + i
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const uint32_t pair = of_token(x.ks, 4 * t + r);
-                u[4 * t + r] = __builtin_fmaf(hi_h(pair), s[r], lo_h(pair) * qz);
-            }
+        for (int i = 0; i < TPL; i++) {
+            float part[CF];
+#pragma unroll
+            for (int j = 0; j < CF; j++) part[j] = s[j * (4 / CF) + i / 4][i % 4];
+            const uint32_t pair = x.ks.get(i);
+            u[i] = __builtin_fmaf(hi_h(pair), pack_lanes<CF>(part), lo_h(pair) * qz);
         }
         if (tail) {
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (i >= left) u[i] = -INFINITY;
+            for (int i = 0; i < TPL; i++)
+                if (first + i >= left) u[i] = -INFINITY;
         }
         float mx = u[0];
 #pragma unroll
-        for (int i = 1; i < 16; i++) mx = fmaxf(mx, u[i]);
+        for (int i = 1; i < TPL; i++) mx = fmaxf(mx, u[i]);
         if (__builtin_amdgcn_ballot_w64((mx - m) * cs > GROW)) {  // some head's maximum moves: all of its lanes'
-            mx = fmaxf(mx, xor16(mx));
-            mx = fmaxf(fmaxf(mx, xor32(mx)), m);
+            mx = fmaxf(head_max<CF>(mx), m);
             const float f = m == mx ? 1.0f : __builtin_amdgcn_exp2f((m - mx) * cs);
             m = mx;
             l *= f;
@@ -370,22 +449,26 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
         const float off = -m * cs;
         uint32_t ph[8], pl[8];  // p step in two f16, in V's token order: 0 2, 1 3 of every four
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
+        for (int t = 0; t < TPL / 4; t++) {
             half_t h[4], e[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(u[4 * t + r], cs, off));
-                const uint32_t pair = of_token(x.vs, 4 * t + r);
+                const uint32_t pair = x.vs.get(4 * t + r);
                 l += p;
                 low = __builtin_fmaf(p, lo_h(pair), low);
                 const float w = p * hi_h(pair);
                 h[r] = (half_t)w;
                 e[r] = (half_t)(w - (float)h[r]);
             }
-            ph[2 * t] = __builtin_bit_cast(uint32_t, half2v{h[0], h[2]});
-            ph[2 * t + 1] = __builtin_bit_cast(uint32_t, half2v{h[1], h[3]});
-            pl[2 * t] = __builtin_bit_cast(uint32_t, half2v{e[0], e[2]});
-            pl[2 * t + 1] = __builtin_bit_cast(uint32_t, half2v{e[1], e[3]});
+            const uint32_t h0 = __builtin_bit_cast(uint32_t, half2v{h[0], h[2]}), h1 = __builtin_bit_cast(uint32_t, half2v{h[1], h[3]});
+            const uint32_t e0 = __builtin_bit_cast(uint32_t, half2v{e[0], e[2]}), e1 = __builtin_bit_cast(uint32_t, half2v{e[1], e[3]});
+#pragma unroll
+            for (int j = 0; j < CF; j++) {
+                const int at = 2 * (j * (4 / CF) + t);
+                ph[at] = part_lanes<CF>(h0, j), ph[at + 1] = part_lanes<CF>(h1, j);
+                pl[at] = part_lanes<CF>(e0, j), pl[at + 1] = part_lanes<CF>(e1, j);
+            }
         }
 #pragma unroll
         for (int s = 0; s < 2; s++) {
@@ -404,7 +487,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
             }
         }
     };
-    Q4Tile<D> x, y;
+    Q4Tile<D, CF> x, y;
     load(wave, x);
     for (int t = wave; t < ntiles; t += 2 * NW) {
         load(t + NW, y);
@@ -414,10 +497,8 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
         step(t + NW, y);
     }
     // The wavefronts' states, joined in order: the maximum (log2 units), sums, outputs.
-    l += xor16(l);
-    l += xor32(l);
-    low += xor16(low);
-    low += xor32(low);
+    l = head_sum<CF>(l);
+    low = head_sum<CF>(low);
     if (l16 < QPG) {
 #pragma unroll
         for (int j = 0; j < D / 32; j++)
@@ -488,13 +569,17 @@ __global__ __launch_bounds__(256) void decode_q4_join(Q4Args a, int qpg) {
     }
 }
 
-// Tokens a chunk. Tables of at most CHUNK_MAX tokens are one chunk (no second launch); longer
-// ones are cut into 256 to CHUNK_MAX tokens, about 8 workgroups a CU at the table's full length, which even out
-// lengths that differ.
+// Tokens a chunk: about two workgroups of 4 wavefronts a CU at the table's full length, which run at one time;
+// 512 at least. A workgroup costs 4 us of latencies before and after its tiles, and a second chunk the
+// join, 5 us: 64 x 128-4096 tokens, 8 kv heads of 128, chunks of 512 / 1024 / 2048 / 4096 51 / 42 / 40 / 35 us, all
+// 4096 77 / 59 / 54 / 50; one sequence of 16384 10.7 / 12.3 / 16.6 / 24.8, 16 x 100-4000 20.7 /
+// 17.4 / 17.7 / 21.7. Tables of at most ONE_CHUNK tokens are one chunk of 8 wavefronts
+// (5 x 20-333 tokens, 4 kv heads of 64, 5.4 us, 4 wavefronts 6.0).
+constexpr int ONE_CHUNK = 1024;
 int chunk_tokens(const TslKernel& k) {
     const int64_t bg = std::max<int64_t>(1, k.dim("B") * k.dim("G")), most = k.dim("MP") * k.dim("P");
-    if (most <= CHUNK_MAX) return CHUNK_MAX;
-    return (int)std::min<int64_t>(std::max<int64_t>(256, (most * bg / (8 * num_cus()) + 255) / 256 * 256), CHUNK_MAX);
+    if (most <= ONE_CHUNK) return ONE_CHUNK;
+    return (int)std::min<int64_t>(std::max<int64_t>(512, (most * bg / (2 * num_cus()) + 255) / 256 * 256), CHUNK_MAX);
 }
 int nchunks(const TslKernel& k) {
     const int64_t most = k.dim("MP") * k.dim("P"), ct = chunk_tokens(k);
@@ -507,7 +592,7 @@ int run_q4(const Q4Args& a, hipStream_t s) {
     if constexpr (D == 16) {
         hipLaunchKernelGGL((decode_q4_any<D, QPG>), grid, dim3(256), 0, s, a);
     } else {
-        if (a.NCH == 1) hipLaunchKernelGGL((decode_q4_mfma<D, QPG, 8>), grid, dim3(512), 0, s, a);
+        if (a.wide) hipLaunchKernelGGL((decode_q4_mfma<D, QPG, 8>), grid, dim3(512), 0, s, a);
         else hipLaunchKernelGGL((decode_q4_mfma<D, QPG, 4>), grid, dim3(256), 0, s, a);
     }
     int r = TSL_LAUNCHED("quant decode_attention");
@@ -564,6 +649,7 @@ int launch_decode_q4(TslKernel& k, const uint64_t* args, hipStream_t s) {
     a.c2 = arg_f32(args[8]) * LOG2E;
     a.B = k.dim("B"), a.H = k.dim("H"), a.G = k.dim("G"), a.NP = k.dim("NP"), a.P = k.dim("P"), a.MP = k.dim("MP");
     a.NCH = nchunks(k), a.CT = chunk_tokens(k), a.pshift = __builtin_ctz((unsigned)a.P);
+    a.wide = (int64_t)a.MP * a.P <= ONE_CHUNK;
     a.part = reinterpret_cast<float*>(k.scratch);
     if (a.B == 0) return 0;
     switch (k.dim("D")) {
