@@ -57,13 +57,33 @@ TSL_DEV void tile_of(int bid, int nwg, int tiles_m, int tiles_n, int G, int& tm,
     tn = (pid % width) / rows;
 }
 
+// 16 k of a row from k (a multiple of 16) on, zeros past K: one load at byte alignment. A chunk that crosses the
+// row's end is the row's last 16 bytes, shifted, so that nothing past a row is read.
+TSL_DEV u32x4 row16(const int8_t* row, int k, int K) {
+    if (k + 16 <= K) return (u32x4) * reinterpret_cast<const u32x4b*>(row + k);
+    u32x4 v = {0, 0, 0, 0};
+    if (k >= K) return v;
+    if (K >= 16) {
+        typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+        u64x2 q = __builtin_bit_cast(u64x2, (u32x4) * reinterpret_cast<const u32x4b*>(row + K - 16));
+        const int drop = 8 * (k + 16 - K);  // 8 .. 120 bits
+        if (drop >= 64) q = u64x2{q[1], 0};
+        const int d = drop & 63;
+        if (d) q = u64x2{q[0] >> d | q[1] << (64 - d), q[1] >> d};
+        return __builtin_bit_cast(u32x4, q);
+    }
+#pragma unroll
+    for (int e = 0; e < 15; e++)
+        if (k + e < K) v[e >> 2] |= (uint32_t)(uint8_t)row[k + e] << (8 * (e & 3));
+    return v;
+}
+
 // Any K and alignment: 16-byte loads at byte alignment into registers, a step ahead, then LDS.
 // 64 x 64 products a workgroup; KG groups of 4 wavefronts take steps g, g + KG, .. of 128 k
 // through two stages of their own, and their sums are added through LDS at the end (4 groups
 // where the tiles make one round on the CUs, else 2: 33 x 2049 x 4095 16.5 / 18.5 us).
 // gate_up's tile holds, for each wavefront column, WN / 2 rows of Wg and their partners of
-// Wu, so a lane has both sums of an output. A chunk that crosses its row's end is the row's last 16 bytes,
-// shifted, so that nothing past a row is read.
+// Wu, so a lane has both sums of an output.
 //
 // Bound by the loads, which straddle lines: 777 x 1155 x 1001 9.5 us (12.5 with one group and each
 // step's loads waited for), 4001 x 4001 x 1001 95.
@@ -98,24 +118,6 @@ __global__ __launch_bounds__(256 * KG) void gemm_i8_any(Gemm8 a) {
     for (int i = 0; i < CA; i++) pa[i] = a.X + (size_t)min(m0 + (i * 256 + t) / KC, a.M - 1) * K;
 #pragma unroll
     for (int i = 0; i < CB; i++) pb[i] = brow((i * 256 + t) / KC);
-    auto chunk = [&](const int8_t* row, int k) {  // 16 k of a row from k on, zeros past K
-        if (k + 16 <= K) return (u32x4) * reinterpret_cast<const u32x4b*>(row + k);
-        u32x4 v = {0, 0, 0, 0};
-        if (k >= K) return v;
-        if (K >= 16) {
-            typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
-            u64x2 q = __builtin_bit_cast(u64x2, (u32x4) * reinterpret_cast<const u32x4b*>(row + K - 16));
-            const int drop = 8 * (k + 16 - K);  // (8 .. 120 bits: the chunk starts at a multiple of 16)
-            if (drop >= 64) q = u64x2{q[1], 0};
-            const int d = drop & 63;
-            if (d) q = u64x2{q[0] >> d | q[1] << (64 - d), q[1] >> d};
-            return __builtin_bit_cast(u32x4, q);
-        }
-#pragma unroll
-        for (int e = 0; e < 15; e++)
-            if (k + e < K) v[e >> 2] |= (uint32_t)(uint8_t)row[k + e] << (8 * (e & 3));
-        return v;
-    };
     i32x4 acc[TM][TN];
 #pragma unroll
     for (int i = 0; i < TM; i++)
@@ -127,9 +129,9 @@ __global__ __launch_bounds__(256 * KG) void gemm_i8_any(Gemm8 a) {
     auto gload = [&](int round) {
         const int k = (round * KG + kg) * BK + c16;
 #pragma unroll
-        for (int i = 0; i < CA; i++) ra[i] = chunk(pa[i], k);
+        for (int i = 0; i < CA; i++) ra[i] = row16(pa[i], k, K);
 #pragma unroll
-        for (int i = 0; i < CB; i++) rb[i] = chunk(pb[i], k);
+        for (int i = 0; i < CB; i++) rb[i] = row16(pb[i], k, K);
     };
     auto sstore = [&](int stage) {
         u32x4* s = ring + stage * STAGE;
@@ -261,6 +263,23 @@ TSL_DEV void store_cols(u16* Y, int N, int m, int n, const u16 (&v)[CNT]) {
     }
 }
 
+// CNT consecutive steps from n (past N the last one's).
+template <int CNT>
+TSL_DEV void load_cols(const float* p, int N, int n, float (&v)[CNT]) {
+    typedef float4v float4u __attribute__((aligned(4)));
+    if (n + CNT <= N) {
+#pragma unroll
+        for (int i = 0; i < CNT / 4; i++) {
+            const float4v t = *reinterpret_cast<const float4u*>(p + n + 4 * i);
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[4 * i + e] = t[e];
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < CNT; c++) v[c] = p[min(n + c, N - 1)];
+    }
+}
+
 // The epilogue of a wavefront's TM x TN tiles: rows m0 + 16 i + l % 16 of Y,
 // columns n0 + 4 TNO (l / 16) .. (TNO: tiles of outputs).
 template <int EPI, int TM, int TN>
@@ -269,22 +288,20 @@ TSL_DEV void store_tiles(const Gemm8& a, int m0, int n0, int lane, const i32x4 (
     constexpr int TNO = DUAL ? TN / 2 : TN, CNT = 4 * TNO;
     const int n = n0 + CNT * (lane >> 4);
     if (n >= a.N) return;
-    float sw[CNT], su[DUAL ? CNT : 1];
+    float sx[TM], sw[CNT], su[DUAL ? CNT : 1];
 #pragma unroll
-    for (int c = 0; c < CNT; c++) {
-        sw[c] = a.SW[min(n + c, a.N - 1)];
-        if constexpr (DUAL) su[c] = a.SW2[min(n + c, a.N - 1)];
-    }
+    for (int i = 0; i < TM; i++) sx[i] = a.SX[min(m0 + 16 * i + (lane & 15), a.M - 1)];
+    load_cols<CNT>(a.SW, a.N, n, sw);
+    if constexpr (DUAL) load_cols<CNT>(a.SW2, a.N, n, su);
 #pragma unroll
     for (int i = 0; i < TM; i++) {
         const int m = m0 + 16 * i + (lane & 15);
         if (m >= a.M) continue;
-        const float sx = a.SX[m];
         u16 v[CNT];
 #pragma unroll
         for (int c = 0; c < CNT; c++) {
-            float f = scaled(acc[i][c / 4][c % 4], sx, sw[c]);
-            if constexpr (DUAL) f = silu_mul(f, scaled(acc[i][TNO + c / 4][c % 4], sx, su[c]));
+            float f = scaled(acc[i][c / 4][c % 4], sx[i], sw[c]);
+            if constexpr (DUAL) f = silu_mul(f, scaled(acc[i][TNO + c / 4][c % 4], sx[i], su[c]));
             v[c] = f2h(f);
         }
         store_cols<CNT>(a.Y, a.N, m, n, v);
@@ -709,45 +726,111 @@ int run_skinny(const Gemm8& a, hipStream_t s) {
     return TSL_LAUNCHED("quant product");
 }
 
-template <int EPI>
-int run_gemm8(const Gemm8& a, hipStream_t s) {
-    if (a.M == 0 || a.N == 0) return 0;
-    constexpr int HALF = EPI == Q_SWIGLU ? 2 : 1;  // gate_up's tiles hold two rows of W a column
-    if (((uint64_t)a.X | (uint64_t)a.W | (uint64_t)a.W2 | (uint64_t)a.K) % 16 != 0 || a.K == 0) {
-        const long tiles = (long)((a.M + 63L) / 64) * ((a.N + 64 / HALF - 1L) / (64 / HALF));
-        if (tiles <= num_cus()) hipLaunchKernelGGL((gemm_i8_any<EPI, 4>), dim3((unsigned)tiles), dim3(1024), 0, s, a);
-        else hipLaunchKernelGGL((gemm_i8_any<EPI, 2>), dim3((unsigned)tiles), dim3(512), 0, s, a);
-        return TSL_LAUNCHED("quant product");
+// X's and W's rows (then Wu's) with K no multiple of 16, copied to rows of Kp bytes (whole steps of 128 k), zeros past
+// K, for the aligned forms: a wavefront a row, 16 bytes a lane.
+__global__ __launch_bounds__(256) void pack_rows_kernel(Gemm8 a, int8_t* __restrict__ out, int Kp, int rows) {
+    for (int i = blockIdx.x * 4 + (threadIdx.x >> 6); i < rows; i += gridDim.x * 4) {
+        int r = i;
+        const int8_t* from = a.X;
+        if (r >= a.M) {
+            r -= a.M, from = a.W;
+            if (r >= a.N) r -= a.N, from = a.W2;
+        }
+        const int8_t* row = from + (size_t)r * a.K;
+        int8_t* to = out + (size_t)i * Kp;
+        for (int k = 16 * (threadIdx.x & 63); k < Kp; k += 1024) *reinterpret_cast<u32x4*>(to + k) = row16(row, k, a.K);
     }
+}
+
+// The aligned forms' costs: the best tile's (K % 128 == 0: the ping-pong too), and the skinny one's (M <= 64).
+struct Plan {
+    int form;  // 0 .. 4: forms[] below, 5: skinny
+    double us;
+};
+template <int EPI>
+Plan plan_aligned(const Gemm8& a) {
+    constexpr int HALF = EPI == Q_SWIGLU ? 2 : 1;  // gate_up's tiles hold two rows of W a column
     const Form forms[] = {{0.18, 2.8, 64, 64 / HALF},    {0.26, 3.2, 64, 128 / HALF},   {0.37, 4.0, 128, 128 / HALF},
                           {0.60, 4.2, 256, 128 / HALF}, {0.91, 6.0, 256, 256 / HALF}};
-    int pick = 0;
-    double best = form_cost(forms[0], a);
-    for (int i = 1; i < 5; i++) {
+    Plan p = {0, form_cost(forms[0], a)};
+    for (int i = 1; i < (a.K % 128 == 0 ? 5 : 4); i++) {
         const double c = form_cost(forms[i], a);
-        if (c < best && (i < 4 || a.K % 128 == 0)) pick = i, best = c;
+        if (c < p.us) p = {i, c};
     }
-    const int mt = (a.M + 15) / 16;
-    if (mt <= 4) {
-        const double blocks = (a.N + 16 / HALF - 1) / (16 / HALF), kb = (16.0 + 16 * mt) * a.K / 1024;
-        if (2.0 + std::max(1.0, blocks / num_cus()) * kb / 54 < best) {
-            switch (mt) {
-                case 1: return run_skinny<EPI, 1, 2>(a, s);
-                case 2: return run_skinny<EPI, 2, 3>(a, s);
-                case 3: return run_skinny<EPI, 3, 2>(a, s);
-                default: return run_skinny<EPI, 4, 2>(a, s);
-            }
-        }
+    if (a.M <= 64) {
+        const double blocks = (a.N + 16 / HALF - 1) / (16 / HALF), kb = (16.0 + (a.M + 15) / 16 * 16) * a.K / 1024;
+        const double c = 2.0 + std::max(1.0, blocks / num_cus()) * kb / 54;
+        if (c < p.us) p = {5, c};
     }
-    switch (pick) {
+    return p;
+}
+
+template <int EPI>
+int run_aligned(const Gemm8& a, hipStream_t s) {
+    switch (plan_aligned<EPI>(a).form) {
         case 0: return run_tile<EPI, 64, 64, 2, 2, 4, 2>(a, s);
         case 1: return run_tile<EPI, 64, 128, 2, 2, 3, 2>(a, s);
         case 2: return run_tile<EPI, 128, 128, 2, 4, 4, 1>(a, s);
         case 3: return run_tile<EPI, 256, 128, 4, 2, 3, 1>(a, s);
+        case 4: {
+            constexpr int OUT = EPI == Q_SWIGLU ? 128 : 256;
+            const long tiles = (long)((a.M + 255L) / 256) * ((a.N + OUT - 1L) / OUT);
+            hipLaunchKernelGGL(gemm_i8_pp<EPI>, dim3((unsigned)tiles), dim3(512), 0, s, a);
+            return TSL_LAUNCHED("quant product");
+        }
     }
-    const long tiles = (long)((a.M + 255L) / 256) * ((a.N + 256 / HALF - 1L) / (256 / HALF));
-    hipLaunchKernelGGL(gemm_i8_pp<EPI>, dim3((unsigned)tiles), dim3(512), 0, s, a);
+    switch ((a.M + 15) / 16) {
+        case 1: return run_skinny<EPI, 1, 2>(a, s);
+        case 2: return run_skinny<EPI, 2, 3>(a, s);
+        case 3: return run_skinny<EPI, 3, 2>(a, s);
+        default: return run_skinny<EPI, 4, 2>(a, s);
+    }
+}
+
+// Whether rows of K no multiple of 16 are copied first (into the handle's scratch): gemm_i8_any takes 4 us and, a
+// step, 0.39 us or its share of 0.7 us a round of the CUs; the copy 4 us and its bytes at 3 TB/s, then the
+// aligned forms (us, any / copied: 4001 x 4001 x 1001 95 / 38, 33 x 2049 x 4095 16.5 / 12.0, 777 x 1155 x 1001 9.5 / 9.8).
+template <int EPI>
+long any_tiles(const Gemm8& a) {
+    constexpr int OUT = EPI == Q_SWIGLU ? 32 : 64;
+    return (long)((a.M + 63L) / 64) * ((a.N + OUT - 1L) / OUT);
+}
+template <int EPI>
+size_t packed_bytes(Gemm8 a) {
+    if (a.K % 16 == 0 || a.M == 0 || a.N == 0) return 0;
+    const double steps = (a.K + 127) / 128, any = 4.0 + steps * std::max(0.39, 0.7 * any_tiles<EPI>(a) / num_cus());
+    a.K = (a.K + 127) / 128 * 128;
+    const size_t bytes = ((size_t)a.M + (EPI == Q_SWIGLU ? 2 : 1) * (size_t)a.N) * a.K;
+    return 4.0 + bytes * 2 / 3e6 + plan_aligned<EPI>(a).us < any ? bytes : 0;
+}
+
+template <int EPI>
+int run_gemm8(Gemm8 a, TslKernel& k, hipStream_t s) {
+    if (a.M == 0 || a.N == 0) return 0;
+    if (k.scratch) {
+        const int kp = (a.K + 127) / 128 * 128, rows = (int)(k.scratch_bytes / kp);
+        int8_t* out = reinterpret_cast<int8_t*>(k.scratch);
+        hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)std::min((rows + 3) / 4, 1 << 16)), dim3(256), 0, s, a, out, kp, rows);
+        if (int r = TSL_LAUNCHED("quant product rows")) return r;
+        a.X = out, a.W = out + (size_t)a.M * kp, a.W2 = a.W2 ? a.W + (size_t)a.N * kp : nullptr, a.K = kp;
+        return run_aligned<EPI>(a, s);
+    }
+    if (((uint64_t)a.X | (uint64_t)a.W | (uint64_t)a.W2 | (uint64_t)a.K) % 16 == 0 && a.K > 0) return run_aligned<EPI>(a, s);
+    const long tiles = any_tiles<EPI>(a);
+    if (tiles <= num_cus()) hipLaunchKernelGGL((gemm_i8_any<EPI, 4>), dim3((unsigned)tiles), dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((gemm_i8_any<EPI, 2>), dim3((unsigned)tiles), dim3(512), 0, s, a);
     return TSL_LAUNCHED("quant product");
+}
+
+template <int EPI>
+int prepare_i8(TslKernel& k, const char* n) {
+    Gemm8 a{};
+    a.M = (int)k.dim("M"), a.N = (int)k.dim(n), a.K = (int)k.dim("K");
+    if (const size_t bytes = packed_bytes<EPI>(a)) {
+        if (tsl_hip_check(hipMalloc(&k.scratch, bytes), ("quant/" + k.name + " scratch").c_str())) return -1;
+        k.scratch_bytes = bytes;
+    }
+    return 0;
 }
 
 int check_i8(const TslKernel& k, const char* n) {
@@ -765,12 +848,15 @@ int check_i8(const TslKernel& k, const char* n) {
 int check_linear_q8(TslKernel& k) { return check_i8(k, "N"); }
 int check_gate_up_q8(TslKernel& k) { return check_i8(k, "F"); }
 
+int prepare_linear_q8(TslKernel& k) { return prepare_i8<Q_LINEAR>(k, "N"); }
+int prepare_gate_up_q8(TslKernel& k) { return prepare_i8<Q_SWIGLU>(k, "F"); }
+
 int launch_linear_q8(TslKernel& k, const uint64_t* a, hipStream_t s) {
     return run_gemm8<Q_LINEAR>({P<int8_t>(a[0]), P<int8_t>(a[2]), nullptr, P<float>(a[1]), P<float>(a[3]), nullptr,
-                                P<u16>(a[4]), (int)k.dim("M"), (int)k.dim("N"), (int)k.dim("K")}, s);
+                                P<u16>(a[4]), (int)k.dim("M"), (int)k.dim("N"), (int)k.dim("K")}, k, s);
 }
 
 int launch_gate_up_q8(TslKernel& k, const uint64_t* a, hipStream_t s) {
     return run_gemm8<Q_SWIGLU>({P<int8_t>(a[0]), P<int8_t>(a[2]), P<int8_t>(a[4]), P<float>(a[1]), P<float>(a[3]),
-                                P<float>(a[5]), P<u16>(a[6]), (int)k.dim("M"), (int)k.dim("F"), (int)k.dim("K")}, s);
+                                P<float>(a[5]), P<u16>(a[6]), (int)k.dim("M"), (int)k.dim("F"), (int)k.dim("K")}, k, s);
 }

@@ -25,6 +25,7 @@ typedef float4v float4u __attribute__((aligned(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x2 u32x2u __attribute__((aligned(1)));
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32u __attribute__((aligned(2)));
 
 TSL_DEV u32x4 load8(const u16* p) { return *reinterpret_cast<const u32x4u*>(p); }
 TSL_DEV float4v load4(const float* p) { return *reinterpret_cast<const float4u*>(p); }
@@ -59,44 +60,47 @@ TSL_DEV double wave_sum64(double x) {
     return (lane_value64(x, 0) + lane_value64(x, 16)) + (lane_value64(x, 32) + lane_value64(x, 48));
 }
 
-// The code of p in a row whose largest magnitude is top > 0: t = 127 p / top
-// from inv = 127 / top, its whole number by adding 1.5 2^23 (f32) or rint
-// (f64). NEAR bounds t's error (127 x 3 half-ulps, doubled); closer to a tie
-// than that, 254 |p| is compared with (2 k + 1) top: p and top of 11 bits
-// (f16) give 19-bit products, exact in f32; products of f32 and f16 (35
-// bits) give 43-bit ones, exact in f64.
+// Codes of values p in a row whose largest magnitude is top > 0: t = 127 p / top from
+// inv = 127 / top, rounded to a whole number by adding 1.5 2^23 (f32; 1.5 2^52 f64), which leaves
+// the code in the sum's low byte. NEAR is above t's error (127 x 2 half-steps of the type);
+// closer to a tie than that, 254 |p| is compared with (2 k + 1) top: p and top
+// of 11 bits (f16) give 19-bit products, exact in f32; products of f32 and f16 (35 bits) give 43-bit
+// ones, exact in f64. One test for 8 values: with one for each, 4096 x 5632 took 15.9 us, 14.0 so (69 MB; the
+// card copies 67 MB in that).
 template <class F>
-struct Code8;
-template <>
-struct Code8<float> {
-    float top, inv;
-    TSL_DEV explicit Code8(float t) : top(t), inv(t > 0.0f ? 127.0f / t : 0.0f) {}
-    TSL_DEV int operator()(float p) const {
-        constexpr float NEAR = 5e-5f;
-        const float t = p * inv;
-        float n = __builtin_rintf(t);
-        if (__builtin_fabsf(t - n) > 0.5f - NEAR) {
-            const float k = __builtin_floorf(__builtin_fabsf(t)), a = 254.0f * __builtin_fabsf(p), b = (2.0f * k + 1.0f) * top;
-            const float m = a > b ? k + 1.0f : a < b ? k : 2.0f * __builtin_rintf(0.5f * (k + 0.5f));
-            n = __builtin_copysignf(m, p);
-        }
-        return (int)n;
+struct Code8 {
+    static constexpr bool WIDE = sizeof(F) == 8;
+    static constexpr F MAGIC = WIDE ? (F)6755399441055744.0 : (F)12582912.0, NEAR = WIDE ? (F)1e-12 : (F)5e-5;
+    F top, inv;
+    TSL_DEV explicit Code8(F t) : top(t), inv(t > 0 ? (F)127 / t : (F)0) {}
+    TSL_DEV int exact(F p) const {
+        const F t = p * inv, n = __builtin_elementwise_roundeven(t), a = __builtin_elementwise_abs(p);
+        if (__builtin_elementwise_abs(t - n) <= (F)0.5 - NEAR) return (int)n;
+        const F k = __builtin_elementwise_floor(__builtin_elementwise_abs(t)), l = (F)254 * a, r = ((F)2 * k + 1) * top;
+        const int m = (int)k + (l > r || (l == r && ((int)k & 1)));
+        return p < 0 ? -m : m;
     }
-};
-template <>
-struct Code8<double> {
-    double top, inv;
-    TSL_DEV explicit Code8(double t) : top(t), inv(t > 0.0 ? 127.0 / t : 0.0) {}
-    TSL_DEV int operator()(double p) const {
-        constexpr double NEAR = 1e-12;
-        const double t = p * inv;
-        double n = __builtin_rint(t);
-        if (__builtin_fabs(t - n) > 0.5 - NEAR) {
-            const double k = __builtin_floor(__builtin_fabs(t)), a = 254.0 * __builtin_fabs(p), b = (2.0 * k + 1.0) * top;
-            const double m = a > b ? k + 1.0 : a < b ? k : 2.0 * __builtin_rint(0.5 * (k + 0.5));
-            n = __builtin_copysign(m, p);
+    TSL_DEV u32x2 operator()(const F (&p)[8]) const {  // eight codes as bytes
+        u32x2 v;
+        F off = 0;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            uint32_t c[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const F u = __builtin_elementwise_fma(p[4 * h + e], inv, MAGIC), n = u - MAGIC;
+                off = __builtin_elementwise_max(off, __builtin_elementwise_abs(__builtin_elementwise_fma(p[4 * h + e], inv, -n)));
+                if constexpr (WIDE) c[e] = (uint32_t)__builtin_bit_cast(uint64_t, u) & 255;
+                else c[e] = __builtin_bit_cast(uint32_t, u) & 255;
+            }
+            v[h] = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
         }
-        return (int)n;
+        if (off > (F)0.5 - NEAR)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                v[h] = (uint32_t)(exact(p[4 * h]) & 255) | (uint32_t)(exact(p[4 * h + 1]) & 255) << 8 |
+                       (uint32_t)(exact(p[4 * h + 2]) & 255) << 16 | (uint32_t)exact(p[4 * h + 3]) << 24;
+        return v;
     }
 };
 
@@ -114,20 +118,15 @@ TSL_DEV T row_reduce(T x, T* red, WaveOp wave, Op op) {
     return x;
 }
 
-// 8 codes as bytes, to row Q at column c of K (8-byte stores at any
-// alignment; element by element where the chunk crosses the row's end).
-TSL_DEV void store_codes(int8_t* q, int c, int K, const int (&n)[8]) {
+// 8 codes to row q at column c of K (8-byte stores at any alignment; byte by byte
+// where the chunk crosses the row's end).
+TSL_DEV void store_codes(int8_t* q, int c, int K, u32x2 v) {
     if (c + 8 <= K) {
-        u32x2 v;
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-            v[h] = (uint32_t)(n[4 * h] & 255) | (uint32_t)(n[4 * h + 1] & 255) << 8 | (uint32_t)(n[4 * h + 2] & 255) << 16 |
-                   (uint32_t)n[4 * h + 3] << 24;
         *reinterpret_cast<u32x2u*>(q + c) = v;
     } else {
 #pragma unroll
         for (int e = 0; e < 8; e++)
-            if (c + e < K) q[c + e] = (int8_t)n[e];
+            if (c + e < K) q[c + e] = (int8_t)(v[e >> 2] >> (8 * (e & 3)));
     }
 }
 
@@ -184,10 +183,10 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void quantize_kernel(const u16
         const float top = bad ? 0.0f : h2f((u16)bits);
         const Code8<float> code(top);
         auto emit = [&](int c, const u32x4& w) {
-            int n[8];
+            float p[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) n[e] = bad ? 0 : code(h2f(half_of(w, e)));
-            if (c < K) store_codes(Q + row * K, c, K, n);
+            for (int e = 0; e < 8; e++) p[e] = h2f(half_of(w, e));
+            if (c < K) store_codes(Q + row * K, c, K, bad ? u32x2{0, 0} : code(p));
         };
         if constexpr (CH > 0) {
 #pragma unroll
@@ -262,10 +261,10 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rmsnorm_q8_kernel(const u
         const bool bad = __builtin_isnan(sum);
         const Code8<double> code(bad ? 0.0 : top);
         auto emit = [&](int c, const float (&rr)[8], const u32x4& ww) {
-            int n[8];
+            double p[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) n[e] = bad ? 0 : code((double)rr[e] * (double)h2f(half_of(ww, e)));
-            if (c < K) store_codes(Q + row * K, c, K, n);
+            for (int e = 0; e < 8; e++) p[e] = (double)rr[e] * (double)h2f(half_of(ww, e));
+            if (c < K) store_codes(Q + row * K, c, K, bad ? u32x2{0, 0} : code(p));
         };
         if constexpr (CH > 0) {
 #pragma unroll
@@ -282,10 +281,13 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rmsnorm_q8_kernel(const u
     }
 }
 
-// kv_write: llm/kv_write's rotated keys and values, into K and V [T, G, D] as there
-// and into the cache in 4 bits. A workgroup per (token, keys or values); D / 4
-// lanes a head: lane j holds channels 2j, 2j + 1 and their rotary partners D/2
-// on, which are the byte pairs j and D/4 + j.
+// kv_write: keys rotated at pos, and values, into K and V [T, G, D] in f16 and into the cache in 4 bits.
+// The rotation is llm/kv_write's, x1 c - x2 s and x2 c + x1 s, in f64 (both products are exact there) and
+// rounded once, so that a key is the f16 nearest to its rotation.
+//
+// A workgroup a token, D / 4 lanes a head: lane j holds channels 2j, 2j + 1 and their rotary
+// partners D/2 on, which are the bytes j and D/4 + j of the cache's row. Bound by its chain of loads
+// (position, slot, rows, tables).
 struct KvArgs {
     const u16* QKV;
     const int *pos, *slot;
@@ -297,35 +299,44 @@ struct KvArgs {
 };
 
 template <int D>
-__global__ __launch_bounds__(256) void kv_write_q4_kernel(KvArgs a) {
+__global__ __launch_bounds__(512) void kv_write_q4_kernel(KvArgs a) {
     constexpr int D2 = D / 2, LPH = D / 4;
-    const int t = blockIdx.x;
-    const bool val = blockIdx.y;  // values (else keys)
+    typedef float float2u __attribute__((ext_vector_type(2), aligned(4)));
+    const int t = blockIdx.x, nt = blockDim.x;
     const int p = a.pos[t], at = a.slot[t];
-    // Rows that name one slot: the last is kept. Every thread looks at its share of the later rows.
+    // Rows that name one slot: the last is kept. Every thread looks at its share of the later rows, 8
+    // loads at a time (2003 tokens 8.7 us with one).
     bool later = false;
-    for (int u = t + 1 + threadIdx.x; u < a.T; u += blockDim.x) later = later || a.slot[u] == at;
+    for (int u = t + 1 + threadIdx.x; u < a.T; u += 8 * nt) {
+        int other[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) other[i] = u + i * nt < a.T ? a.slot[u + i * nt] : -1;
+#pragma unroll
+        for (int i = 0; i < 8; i++) later = later || other[i] == at;
+    }
     const bool keep = !__syncthreads_or(later) && at >= 0 && at < a.NS;
     const int lane = threadIdx.x % LPH;
     const long page = keep ? at / a.P : 0;
     const int off = keep ? at % a.P : 0;
-    // Every thread goes round as often (the reductions below take whole wavefronts).
-    const int nh = blockDim.x / LPH;
-    for (int g0 = 0; g0 < a.G; g0 += nh) {
-        const int g = g0 + threadIdx.x / LPH;
-        const bool live = g < a.G;
-        const u16* x = a.QKV + (long)t * a.W + (a.W - (val ? 1L : 2L) * a.G * D) + (long)(live ? g : 0) * D;
-        u16 y[4];
-        if (val) {
-#pragma unroll
-            for (int i = 0; i < 2; i++) y[i] = x[2 * lane + i], y[2 + i] = x[D2 + 2 * lane + i];
-        } else {
-            const bool pin = p >= 0 && p < a.NPOS;
+    // Head h: key h, or value h - G. Every thread goes round as often (the reductions take whole wavefronts).
+    for (int h0 = 0; h0 < 2 * a.G; h0 += nt / LPH) {
+        const int h = h0 + threadIdx.x / LPH;
+        const bool live = h < 2 * a.G, val = h >= a.G;
+        const int g = val ? h - a.G : h;
+        const u16* x = a.QKV + (long)t * a.W + (a.W - 2L * a.G * D) + (long)(live ? h : 0) * D + 2 * lane;
+        const uint32_t xa = *reinterpret_cast<const u32u*>(x), xb = *reinterpret_cast<const u32u*>(x + D2);
+        u16 y[4] = {(u16)xa, (u16)(xa >> 16), (u16)xb, (u16)(xb >> 16)};
+        if (!val) {
+            float2u c = {0.0f, 0.0f}, s = {0.0f, 0.0f};
+            if (p >= 0 && p < a.NPOS) {
+                c = *reinterpret_cast<const float2u*>(a.Cs + (long)p * D2 + 2 * lane);
+                s = *reinterpret_cast<const float2u*>(a.Sn + (long)p * D2 + 2 * lane);
+            }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const float c = pin ? a.Cs[(long)p * D2 + 2 * lane + i] : 0.0f;
-                const float s = pin ? a.Sn[(long)p * D2 + 2 * lane + i] : 0.0f;
-                rope_rotate(h2f(x[2 * lane + i]), h2f(x[D2 + 2 * lane + i]), c, s, y[i], y[2 + i]);
+                const double x1 = h2f(y[i]), x2 = h2f(y[2 + i]), ci = c[i], si = s[i];
+                y[i] = __builtin_bit_cast(u16, (half_t)(x1 * ci - x2 * si));
+                y[2 + i] = __builtin_bit_cast(u16, (half_t)(x2 * ci + x1 * si));
             }
         }
         float lo = INFINITY, hi = -INFINITY;
@@ -339,7 +350,7 @@ __global__ __launch_bounds__(256) void kv_write_q4_kernel(KvArgs a) {
         }
         if (bad) lo = -INFINITY, hi = INFINITY;
         // Over the head's lanes (LPH = 4 .. 32, aligned).
-        auto both = [&](float l, float h) { lo = fminf(lo, l), hi = fmaxf(hi, h); };
+        auto both = [&](float l, float u) { lo = fminf(lo, l), hi = fmaxf(hi, u); };
         both(dpp<DPP_XOR1>(lo), dpp<DPP_XOR1>(hi));
         both(dpp<DPP_XOR2>(lo), dpp<DPP_XOR2>(hi));
         if constexpr (LPH >= 8) both(dpp<DPP_HALF_MIRROR>(lo), dpp<DPP_HALF_MIRROR>(hi));
@@ -355,15 +366,15 @@ __global__ __launch_bounds__(256) void kv_write_q4_kernel(KvArgs a) {
             const double d = bad ? 0.0 : (double)h2f(y[i]) - (double)lo, q = d * inv;
             double r = __builtin_rint(q);
             if (fabs(q - r) > 0.5 - 1e-12) {
-                const double k = __builtin_floor(q), l = 30.0 * d, h = (2.0 * k + 1.0) * range;
-                r = l > h ? k + 1.0 : l < h ? k : 2.0 * __builtin_rint(0.5 * (k + 0.5));
+                const double k = __builtin_floor(q), l = 30.0 * d, u = (2.0 * k + 1.0) * range;
+                r = l > u ? k + 1.0 : l < u ? k : 2.0 * __builtin_rint(0.5 * (k + 0.5));
             }
             n[i] = (int)r;
         }
         if (!live) continue;
-        u16* out = (val ? a.V : a.K) + ((long)t * a.G + g) * D;
-#pragma unroll
-        for (int i = 0; i < 2; i++) out[2 * lane + i] = y[i], out[D2 + 2 * lane + i] = y[2 + i];
+        u16* out = (val ? a.V : a.K) + ((long)t * a.G + g) * D + 2 * lane;
+        *reinterpret_cast<u32u*>(out) = (uint32_t)y[0] | (uint32_t)y[1] << 16;
+        *reinterpret_cast<u32u*>(out + D2) = (uint32_t)y[2] | (uint32_t)y[3] << 16;
         if (!keep) continue;
         const long head = page * a.G + g;
         const uint8_t b0 = (uint8_t)(n[0] | n[1] << 4), b1 = (uint8_t)(n[2] | n[3] << 4);
@@ -387,16 +398,29 @@ __global__ __launch_bounds__(256) void kv_write_q4_kernel(KvArgs a) {
 // Workgroups of rows: at most 2^20 of them, which go on to later rows.
 unsigned row_grid(long rows, int rpb) { return (unsigned)std::min((rows + rpb - 1) / rpb, 1L << 20); }
 
-// The threads and register chunks of a row of K: f(NT, CH).
-template <class F>
+// The threads and register chunks of a row of K: f(NT, CH). CHUNKS: the most chunks a thread holds;
+// quantize's rows stream faster with four loads a thread in flight (4096 x 5632 256 threads of 4 / 384 of 2 15.9 /
+// 18.6 us), the norms', three times the registers, with two (512 x 8192 256 of 4 / 512 of 2 9.8 / 8.5).
+template <int CHUNKS, class F>
 void by_length(int K, F f) {
-    if (K <= 512) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 1>{});
-    else if (K <= 1024) f(std::integral_constant<int, 64>{}, std::integral_constant<int, 2>{});
-    else if (K <= 2048) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 1>{});
-    else if (K <= 4096) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
-    else if (K <= 8192) f(std::integral_constant<int, 256>{}, std::integral_constant<int, 4>{});
-    else if (K <= 16384) f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 2>{});
-    else f(std::integral_constant<int, 1024>{}, std::integral_constant<int, 0>{});
+    auto go = [&](auto nt, auto ch) { f(nt, ch); };
+#define Q_ROWS(NT, CH) go(std::integral_constant<int, NT>{}, std::integral_constant<int, CH>{})
+    if (K <= 512) Q_ROWS(64, 1);
+    else if (K <= 1024) Q_ROWS(64, 2);
+    else if (K <= 2048) Q_ROWS(256, 1);
+    else if (K <= 4096) Q_ROWS(256, 2);
+    else if constexpr (CHUNKS == 4) {
+        if (K <= 8192) Q_ROWS(256, 4);
+        else if (K <= 16384) Q_ROWS(512, 4);
+        else Q_ROWS(1024, 0);
+    } else {
+        if (K <= 6144) Q_ROWS(384, 2);
+        else if (K <= 8192) Q_ROWS(512, 2);
+        else if (K <= 12288) Q_ROWS(768, 2);
+        else if (K <= 16384) Q_ROWS(1024, 2);
+        else Q_ROWS(1024, 0);
+    }
+#undef Q_ROWS
 }
 
 int check_rows(const TslKernel& k, const char* rows, const char* cols) {
@@ -409,7 +433,7 @@ template <bool ADD>
 int run_rmsnorm_q8(TslKernel& k, const u16* X, const uint64_t* a, hipStream_t s) {
     const int M = k.dim("T"), K = k.dim("Dm");
     if (M == 0) return 0;
-    by_length(K, [&](auto nt, auto ch) {
+    by_length<2>(K, [&](auto nt, auto ch) {
         constexpr int NT = decltype(nt)::value, CH = decltype(ch)::value, RPB = NT < 256 ? 256 / NT : 1;
         hipLaunchKernelGGL((rmsnorm_q8_kernel<NT, CH, ADD>), dim3(row_grid(M, RPB)), dim3(NT * RPB), 0, s, X,
                            P<float>(a[0]), P<u16>(a[1]), P<int8_t>(a[2]), P<float>(a[3]), M, K, arg_f32(a[4]));
@@ -428,7 +452,7 @@ int check_rmsnorm_q8(TslKernel& k) {
 int launch_quantize(TslKernel& k, const uint64_t* a, hipStream_t s) {
     const int M = k.dim("M"), K = k.dim("K");
     if (M == 0) return 0;
-    by_length(K, [&](auto nt, auto ch) {
+    by_length<4>(K, [&](auto nt, auto ch) {
         constexpr int NT = decltype(nt)::value, CH = decltype(ch)::value, RPB = NT < 256 ? 256 / NT : 1;
         hipLaunchKernelGGL((quantize_kernel<NT, CH>), dim3(row_grid(M, RPB)), dim3(NT * RPB), 0, s, P<u16>(a[0]),
                            P<int8_t>(a[1]), P<float>(a[2]), M, K);
@@ -459,8 +483,8 @@ int check_kv_write_q4(TslKernel& k) {
     if (int r = check_cache_q4(k)) return r;
     if (k.dim("W") < 2 * k.dim("G") * k.dim("D"))
         return tsl_fail(-2, "quant/kv_write: rows of W = " + std::to_string(k.dim("W")) + " hold no 2 G D keys and values");
-    if (k.dim("T") > INT_MAX || k.dim("W") > INT_MAX || k.dim("NPOS") > INT_MAX)
-        return tsl_fail(-2, "quant/kv_write: sizes must be below 2^31");
+    if (k.dim("T") > (1 << 23) || k.dim("W") > INT_MAX || k.dim("NPOS") > INT_MAX)
+        return tsl_fail(-2, "quant/kv_write: at most 2^23 tokens, and sizes below 2^31");
     return 0;
 }
 
@@ -472,12 +496,13 @@ int launch_kv_write_q4(TslKernel& k, const uint64_t* a, hipStream_t s) {
     r.Kc = P<uint8_t>(a[5]), r.Vc = P<uint8_t>(a[6]), r.Ks = P<u16>(a[7]), r.Vs = P<u16>(a[8]);
     r.K = P<u16>(a[9]), r.V = P<u16>(a[10]);
     if (r.T == 0) return 0;
-    const int D = k.dim("D"), lanes = r.G * (D / 4) > 256 ? 256 : (r.G * (D / 4) + 63) / 64 * 64;
+    const int D = k.dim("D");
+    const int lanes = (int)std::min<long>(512, (2L * r.G * (D / 4) + 63) / 64 * 64);
     switch (D) {
-        case 16: hipLaunchKernelGGL(kv_write_q4_kernel<16>, dim3(r.T, 2), dim3(lanes), 0, s, r); break;
-        case 32: hipLaunchKernelGGL(kv_write_q4_kernel<32>, dim3(r.T, 2), dim3(lanes), 0, s, r); break;
-        case 64: hipLaunchKernelGGL(kv_write_q4_kernel<64>, dim3(r.T, 2), dim3(lanes), 0, s, r); break;
-        default: hipLaunchKernelGGL(kv_write_q4_kernel<128>, dim3(r.T, 2), dim3(lanes), 0, s, r); break;
+        case 16: hipLaunchKernelGGL(kv_write_q4_kernel<16>, dim3(r.T), dim3(lanes), 0, s, r); break;
+        case 32: hipLaunchKernelGGL(kv_write_q4_kernel<32>, dim3(r.T), dim3(lanes), 0, s, r); break;
+        case 64: hipLaunchKernelGGL(kv_write_q4_kernel<64>, dim3(r.T), dim3(lanes), 0, s, r); break;
+        default: hipLaunchKernelGGL(kv_write_q4_kernel<128>, dim3(r.T), dim3(lanes), 0, s, r); break;
     }
     return TSL_LAUNCHED("quant kv_write");
 }

@@ -71,6 +71,8 @@ int check_linear_q8(TslKernel&);
 int check_gate_up_q8(TslKernel&);
 int check_decode_q4(TslKernel&);
 int prepare_decode_q4(TslKernel&);
+int prepare_linear_q8(TslKernel&);
+int prepare_gate_up_q8(TslKernel&);
 
 // Compute units of the current device (cached; 256 if the query fails).
 int num_cus() {
@@ -205,10 +207,10 @@ std::vector<KernelDef> g_defs = {
      launch_add_rmsnorm_q8, nullptr, check_rmsnorm_q8},
     // llm/linear and llm/gate_up of such rows: X SX, W SW.
     {"quant", "linear", "X: i8[M, K], SX: f32[M], W: i8[N, K], SW: f32[N], Y: f16[M, N]", "", "", launch_linear_q8,
-     nullptr, check_linear_q8},
+     prepare_linear_q8, check_linear_q8},
     {"quant", "gate_up",
      "X: i8[M, K], SX: f32[M], Wg: i8[F, K], SG: f32[F], Wu: i8[F, K], SU: f32[F], Y: f16[M, F]", "", "",
-     launch_gate_up_q8, nullptr, check_gate_up_q8},
+     launch_gate_up_q8, prepare_gate_up_q8, check_gate_up_q8},
     // llm/kv_write and llm/decode_attention with the cache in 4 bits: codes two
     // a byte, and (lowest value, step) of each token and kv head.
     {"quant", "kv_write",

@@ -220,16 +220,26 @@ def _write_case(rng, t, h, g, d, p, pages, w_extra=0):
             np.full((t, g, d), 7, np.float16), np.full((t, g, d), 7, np.float16)], (kn, vn)
 
 
-def _check_write(case, codes, order=None):
-    """K and V are llm/kv_write's bits; the cache holds their 4-bit forms, and elsewhere what it held."""
+def _check_write(case, codes):
+    """K is the f16 nearest to the rotation in f64 (and so within a step of llm/kv_write's), V the values' bits; the
+    cache holds their 4-bit forms, and elsewhere what it held."""
     qkv, pos, slot, cos, sin, kc, vc, ks, vs, k, v = case
     kn, vn = (c.copy() for c in codes)
     t, g, d = k.shape
     pages, _, p, _ = kc.shape
     got = run("kv_write", case, outputs=range(5, 11))
+    kv = qkv[:, qkv.shape[1] - 2 * g * d:].reshape(t, 2, g, d)
+    there = ((pos >= 0) & (pos < len(cos)))[:, None, None]
+    c, s = (np.where(there, x[np.clip(pos, 0, len(cos) - 1)][:, None].astype(np.float64), 0.0) for x in (cos, sin))
+    x1, x2 = kv[:, 0, :, :d // 2].astype(np.float64), kv[:, 0, :, d // 2:].astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        want_k = np.concatenate([x1 * c - x2 * s, x2 * c + x1 * s], -1).astype(np.float16)
+    np.testing.assert_array_equal(got[9], want_k)
+    np.testing.assert_array_equal(got[10].view(np.uint16), kv[:, 1].view(np.uint16))
     wide = np.zeros((pages * p, g, d), np.float16)
     ref = T.run("llm", "kv_write", [qkv, pos, slot, cos, sin, wide, wide, k, v], outputs=[7, 8])
-    np.testing.assert_array_equal(got[9].view(np.uint16), ref[7].view(np.uint16))
+    # (llm/kv_write rounds one product to f32 first: half an f32 step of it, then f16's half step)
+    np.testing.assert_allclose(ref[7].astype(np.float64), want_k.astype(np.float64), rtol=2 * H, atol=2.0 ** -24 + F * 8)
     np.testing.assert_array_equal(got[10].view(np.uint16), ref[8].view(np.uint16))
     ks, vs = ks.copy(), vs.copy()
     for x, n, pair in ((got[9], kn, ks), (got[10], vn, vs)):
