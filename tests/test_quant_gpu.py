@@ -207,6 +207,99 @@ def test_products_of_extreme_rows():
         np.testing.assert_array_equal(y, want)
 
 
+@pytest.mark.parametrize("m,n,k", [(70, 2300, 1000), (300, 1600, 4095), (5, 48, 2001)])
+def test_linear_at_any_alignment(m, n, k):
+    # Operands that begin at odd addresses, and Y at an odd f16: the bits are those of aligned ones.
+    _say("linear unaligned", m, n, k)
+    rng = np.random.default_rng(m + n + k)
+    (x, sx), (w, sw) = _rows(rng, m, k), _rows(rng, n, k)
+    want = R.product(x, sx, w, sw).astype(np.float16)
+    kern = T.kernel("quant", "linear", [x.shape, sx.shape, w.shape, sw.shape, (m, n)])
+    for off in (1, 4, 16):
+        bx, bw, by = T.alloc(x.nbytes + 32), T.alloc(w.nbytes + 32), T.alloc(2 * m * n + 64)
+        bsx, bsw = T.tensor(sx), T.tensor(sw)
+        T.write(bx, off, x)
+        T.write(bw, off, w)
+        T.launch(kern, [T.Buf(bx.ptr + off, x.nbytes), bsx, T.Buf(bw.ptr + off, w.nbytes), bsw, T.Buf(by.ptr + 2, 2 * m * n)])
+        got = T.read(by, 0, 2 * m * n + 64).view(np.float16)
+        np.testing.assert_array_equal(got[1:1 + m * n].reshape(m, n).view(np.uint16), want.view(np.uint16))
+        assert not got[0] and not got[1 + m * n:].any()  # nothing beside Y
+        for b in (bx, bw, by, bsx, bsw):
+            T.free(b)
+
+
+@pytest.mark.parametrize("m", [3, 200])
+def test_linear_of_weights_past_4_gib(m):
+    # 40000 rows of 131056: the last rows' offsets pass 32 bits. Zeros but for three rows.
+    _say("linear past 4 GiB", m)
+    n, k = 40000, 131056
+    rng = np.random.default_rng(m)
+    (x, sx), (rows, srows) = _rows(rng, m, k), _rows(rng, 3, k)
+    at, sw = np.array([0, 32800, n - 1]), np.ones(n, np.float32)
+    sw[at] = srows
+    bw, by = T.alloc(n * k), T.alloc(2 * m * n)
+    for i, r in zip(at, rows):
+        T.write(bw, int(i) * k, r)
+    bx, bsx, bsw = T.tensor(x), T.tensor(sx), T.tensor(sw)
+    T.launch(T.kernel("quant", "linear", [x.shape, sx.shape, (n, k), sw.shape, (m, n)]), [bx, bsx, bw, bsw, by])
+    y = T.read_array(by, np.float16, (m, n))
+    np.testing.assert_array_equal(y[:, at].view(np.uint16), R.product(x, sx, rows, srows).astype(np.float16).view(np.uint16))
+    y[:, at] = 0
+    assert not y.any()
+    for b in (bw, by, bx, bsx, bsw):
+        T.free(b)
+
+
+@pytest.mark.parametrize("m,n,k,launches", [(400, 2100, 1001, 1), (1500, 2100, 2001, 2)])
+def test_products_share_a_handle_in_a_graph(m, n, k, launches):
+    # Two products of one handle in a graph, replayed with eager launches of other operands between; the second size's
+    # rows are copied first, into the handle's scratch.
+    _say("linear twice in a graph", m, n, k)
+    rng = np.random.default_rng(4)
+    kern, sets = T.kernel("quant", "linear", [(m, k), (m,), (n, k), (n,), (m, n)]), []
+    for _ in range(3):
+        (x, sx), (w, sw) = _rows(rng, m, k), _rows(rng, n, k)
+        sets.append(([T.tensor(v) for v in (x, sx, w, sw)] + [T.alloc(2 * m * n)], R.product(x, sx, w, sw).astype(np.float16)))
+    T.capture_begin()
+    for args, _ in sets[:2]:
+        T.launch(kern, args)
+    graph = T.capture_end()
+    assert T.graph_nodes(graph) == {"kernel": 2 * launches, "memset": 0, "memcpy": 0, "other": 0}
+    for _ in range(3):
+        for args, _ in sets:
+            T.fill_nan(args[4])
+        T.launch(kern, sets[2][0])
+        T.replay(graph)
+        T.launch(kern, sets[2][0])
+        for args, want in sets:
+            np.testing.assert_array_equal(T.read_array(args[4], np.float16, (m, n)).view(np.uint16), want.view(np.uint16))
+    for args, _ in sets:
+        for b in args:
+            T.free(b)
+
+
+@pytest.mark.parametrize("name", ["quantize", "rmsnorm"])
+def test_rows_end_where_they_end(name):
+    # Codes at odd addresses, bytes before and after untouched; rows of every tail length.
+    _say("row guards", name)
+    rng = np.random.default_rng(8)
+    for m, k in ((3, 9), (2, 63), (5, 517), (2, 1031), (2, 2055), (1, 4101), (2, 6150), (1, 9001), (1, 16391), (1, 33001)):
+        x = rng.standard_normal((m, k)).astype(np.float16)
+        q, s = T.tensor(np.full(m * k + 64, 99, np.int8)), T.tensor(np.full(m + 2, 7, np.float32))
+        out, sc = T.Buf(q.ptr + 33, m * k), T.Buf(s.ptr + 4, 4 * m)
+        if name == "quantize":
+            bufs = [T.tensor(x)]
+            T.launch(T.kernel("quant", name, [(m, k), (m, k), (m,)]), bufs + [out, sc])
+        else:
+            bufs = [T.tensor(x.astype(np.float32)), T.tensor(np.ones(k, np.float16))]
+            T.launch(T.kernel("quant", name, [(m, k), (k,), (m, k), (m,)]), bufs + [out, sc, T.F32(1e-5)])
+        got, gs = T.read(q, 0, m * k + 64).view(np.int8), T.read_array(s, np.float32, (m + 2,))
+        np.testing.assert_array_equal(got[33:33 + m * k].reshape(m, k), R.rows8(x)[0])
+        assert (got[:33] == 99).all() and (got[33 + m * k:] == 99).all() and gs[0] == 7 and gs[-1] == 7
+        for b in bufs + [q, s]:
+            T.free(b)
+
+
 # ---------------------------------------------------------------- the 4-bit cache
 
 def _write_case(rng, t, h, g, d, p, pages, w_extra=0):
@@ -362,6 +455,38 @@ def test_decode_attention_far_scores(d, h, g):
     _close(_attend(*case), *case)
     case[0][0] = 0
     _close(_attend(*case), *case)
+
+
+def test_a_cache_past_4_gib():
+    # 600000 pages of 8 heads of 128: codes of 4.9 GB each. Tokens written to its last pages and read from there.
+    _say("cache past 4 GiB")
+    rng = np.random.default_rng(12)
+    h, g, d, p, pages, t = 16, 8, 128, 16, 600000, 40
+    kc, vc, ks, vs = (T.alloc(pages * g * p * n) for n in (d // 2, d // 2, 4, 4))
+    qkv = rng.standard_normal((t, 2 * g * d)).astype(np.float16)
+    where = np.array([pages - 1, 3, pages - 2], np.int32)  # tokens 0 .. 15, 16 .. 31, 32 .. 39
+    slot = (where[np.arange(t) // p] * p + np.arange(t) % p).astype(np.int32)
+    one, zero = np.ones((1, d // 2), np.float32), np.zeros((1, d // 2), np.float32)
+    k, v, q, o = T.alloc(2 * t * g * d), T.alloc(2 * t * g * d), rng.standard_normal((1, h, d)).astype(np.float16), T.alloc(2 * h * d)
+    cache = [(pages, g, p, d // 2), (pages, g, 1, d // 2, 16), (pages, g, p, 2), (pages, g, p, 2)]
+    ins = [T.tensor(x) for x in (qkv, np.zeros(t, np.int32), slot, one, zero, q, where[None], np.array([t], np.int32))]
+    T.launch(T.kernel("quant", "kv_write", [qkv.shape, (t,), (t,), one.shape, zero.shape, *cache, (t, g, d), (t, g, d)]),
+             ins[:5] + [kc, vc, ks, vs, k, v])
+    T.launch(T.kernel("quant", "decode_attention", [q.shape, *cache, (1, 3), (1,), q.shape]),
+             [ins[5], kc, vc, ks, vs, ins[6], ins[7], o, T.F32(0.09)])
+    x = qkv.reshape(t, 2, g, d)  # (not turned: position 0)
+    kn, kp = R.heads4(x[:, 0])
+    vn, vp = R.heads4(x[:, 1])
+    small = [np.zeros((3, g, p, *a.shape[2:]), a.dtype) for a in (kn, vn, kp, vp)]
+    for a, b in zip(small, (kn, vn, kp, vp)):
+        for i in range(t):
+            a[i // p, :, i % p] = b[i]
+    _close(T.read_array(o, np.float16, q.shape).astype(np.float64), q, *small[:2], small[2], small[3], np.array([[0, 1, 2]]),
+           np.array([t]), 0.09)
+    at = ((pages - 2) * g + 5) * p * (d // 2)
+    np.testing.assert_array_equal(T.read(kc, at, p * d // 2).reshape(p, -1), R.pack_k(small[0])[2, 5])
+    for b in (kc, vc, ks, vs, k, v, o, *ins):
+        T.free(b)
 
 
 def test_decode_attention_repeats_and_replays_its_bits():
