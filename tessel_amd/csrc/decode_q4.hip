@@ -238,6 +238,12 @@ struct Pairs {
         for (int i = 0; i < 4 / CF; i++) w[i].load(q + 16 * i);
     }
     TSL_DEV uint32_t get(int i) const { return w[i / 4].w[i % 4]; }
+    TSL_DEV uint32_t most() const {  // the largest step's bits (in the upper half)
+        uint32_t x = 0;
+#pragma unroll
+        for (int i = 0; i < 16 / CF; i++) x = max(x, w[i / 4].w[i % 4] & 0x7fff0000u);
+        return x;
+    }
     TSL_DEV void drop(int first, int left, bool all) {  // tokens first + .. at left and past it, or all of them
 #pragma unroll
         for (int i = 0; i < 16 / CF; i++)
@@ -249,6 +255,7 @@ struct Pairs<1> {
     uint32_t w;
     TSL_DEV void load(const u16* p, long block, int l16) { w = reinterpret_cast<const uint32_t*>(p)[block * 16 + l16]; }
     TSL_DEV uint32_t get(int i) const { return of_token(w, i); }
+    TSL_DEV uint32_t most() const { return w & 0x7fff0000u; }
     TSL_DEV void drop(int, int left, bool all) {
         if (all || (int)(threadIdx.x & 15) >= left) w = 0;
     }
@@ -301,7 +308,9 @@ TSL_DEV float head_sum(float x) {
 template <int D, int QPG, int NW>
 __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q4_mfma(Q4Args a) {
     constexpr int KW = D / 32, NT = D / 16, CB = D / 8;  // words of a K row a lane; channel tiles; their bytes
-    constexpr float GROW = 2.0f;                        // p <= 2^GROW: p step stays in f16
+    // p = 2^(cs (u - m) + lift): m a maximum of u that may grow by 2^GROW before it is moved, lift such that p step
+    // stays below 2^15 for the largest step met: small values keep their f16 bits too.
+    constexpr float GROW = 2.0f;
     // Few query heads leave most of the 16 columns empty: the scores of four (two)
     // of a lane's tiles are packed onto the row's lanes, 16 / CF a lane, for the softmax.
     constexpr int CF = QPG <= 4 ? 4 : QPG == 8 ? 2 : 1, TPL = 16 / CF;
@@ -395,7 +404,9 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
         for (int j = 0; j < KW; j++) x.v[j].load(vp + j * 256);
     };
 
-    float m = -INFINITY, l = 0.0f, low = 0.0f;  // running maximum of u; sums of p and p low (this lane's tokens)
+    float m = -INFINITY, l = 0.0f, low = 0.0f;  // maximum of u; sums of p and p low (this lane's tokens)
+    float lift = 0.0f;                         // (these two of the wavefront)
+    uint32_t most = 0;                         // steps below this bound need no other lift
     float4v acc[NT];
 #pragma unroll
     for (int i = 0; i < NT; i++) acc[i] = float4v{};
@@ -437,16 +448,27 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
         float mx = u[0];
 #pragma unroll
         for (int i = 1; i < TPL; i++) mx = fmaxf(mx, u[i]);
-        if (__builtin_amdgcn_ballot_w64((mx - m) * cs > GROW)) {  // some head's maximum moves: all of its lanes'
+        // Some head's maximum moves, or a step passes the bound: all lanes of the heads together.
+        const uint32_t sm = x.vs.most();
+        if (__builtin_amdgcn_ballot_w64((mx - m) * cs > GROW || sm >= most)) {
             mx = fmaxf(head_max<CF>(mx), m);
-            const float f = m == mx ? 1.0f : __builtin_amdgcn_exp2f((m - mx) * cs);
+            float by = m == mx ? 0.0f : (m - mx) * cs;
             m = mx;
+            const float step = wave_max(h2f((u16)(sm >> 16)));  // (NaN and infinite steps have no lift of their own)
+            if (__builtin_amdgcn_ballot_w64(sm >= most)) {
+                const int e = max(min(step > 0.0f && step <= 65504.0f ? __builtin_amdgcn_frexp_expf(step) : -11, 16), -11);
+                const float to = 13.0f - e;  // 2^(lift + GROW + e) = 2^15
+                by += to - lift;
+                lift = to;
+                most = e < 16 ? (uint32_t)(e + 15) << 26 : 0x7c000000u;  // 2^e as f16 bits, in the upper half
+            }
+            const float f = __builtin_amdgcn_exp2f(by);
             l *= f;
             low *= f;
 #pragma unroll
             for (int i = 0; i < NT; i++) acc[i] *= f;
         }
-        const float off = -m * cs;
+        const float off = lift - m * cs;
         uint32_t ph[8], pl[8];  // p step in two f16, in V's token order: 0 2, 1 3 of every four
 #pragma unroll
         for (int t = 0; t < TPL / 4; t++) {
@@ -508,7 +530,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
                 for (int r = 0; r < 4; r++)
                     red[wave][l16][2 * (16 * j + 4 * g4 + r) + e] =
                         __builtin_fmaf(acc[2 * j + e][r], e ? 0x1p20f : 0x1p24f, low);
-        if (g4 == 0) red[wave][l16][D] = m * cs, red[wave][l16][D + 1] = l;
+        if (g4 == 0) red[wave][l16][D] = m * cs - lift, red[wave][l16][D + 1] = l;
     }
     __syncthreads();
     const int active = min(NW, ntiles);

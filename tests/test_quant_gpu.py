@@ -457,6 +457,49 @@ def test_decode_attention_far_scores(d, h, g):
     _close(_attend(*case), *case)
 
 
+@pytest.mark.parametrize("d,h,g", [(16, 4, 2), (32, 8, 8), (64, 16, 1), (128, 8, 1)])
+def test_decode_attention_scales_and_spoilt_queries(d, h, g):
+    # A negative scale turns the order over; 0 makes a mean of the values. A query that holds an infinity or a NaN
+    # spoils its own head, one of the largest and smallest f16 magnitudes none.
+    _say("decode_attention scales", d)
+    rng = np.random.default_rng(d + 3)
+    case = _attention_case(rng, 3, h, g, d, 16, [70, 1100, 9])
+    for scale in (-0.25, 0.0, 1e-30):
+        case[7] = float(np.float32(scale))
+        _close(_attend(*case), *case)
+    case[7] = 2.0 ** -20
+    q = case[0]
+    q[1, 1, 2] = 65504
+    q[1, 1, 3:6] = np.float16(6e-8)
+    _close(_attend(*case), *case)
+    q[0, 0, 1], q[1, 2, d - 1], q[2, h - 1, 0] = np.inf, np.nan, -np.inf
+    got = _attend(*case)
+    want = np.zeros((3, h), bool)
+    want[0, 0] = want[1, 2] = want[2, h - 1] = True
+    np.testing.assert_array_equal(np.isnan(got), np.broadcast_to(want[:, :, None], got.shape))
+    q[0, 0, 1] = q[1, 2, d - 1] = q[2, h - 1, 0] = 0
+    clean = _attend(*case)
+    np.testing.assert_array_equal(got[~want], clean[~want])
+
+
+@pytest.mark.parametrize("d,h,g", [(16, 4, 2), (32, 16, 1), (64, 8, 4), (128, 8, 1)])
+def test_decode_attention_small_and_large_values(d, h, g):
+    # Values of 1e-5 to 6e4, alone and on neighbouring pages: probabilities keep their bits beside any step.
+    _say("decode_attention values", d)
+    rng = np.random.default_rng(d + 4)
+    for factor in (2e-5, 1e-3, 1000.0, None):
+        case = _attention_case(rng, 3, h, g, d, 16, [1300, 70, 400])
+        vs = case[4].astype(np.float64)
+        vs *= factor if factor else rng.choice([1e-4, 1.0, 3000.0], (len(vs), 1, 1, 1))
+        case[4] = vs.astype(np.float16)
+        _close(_attend(*case), *case)
+    case[4][:] = np.array([-65504, 8736], np.float16)  # the widest head
+    case[2] = np.minimum(case[2], 14)
+    _close(_attend(*case), *case)
+    case[4][:] = np.array([6e-8, 0], np.float16)       # equal values
+    _close(_attend(*case), *case)
+
+
 def test_a_cache_past_4_gib():
     # 600000 pages of 8 heads of 128: codes of 4.9 GB each. Tokens written to its last pages and read from there.
     _say("cache past 4 GiB")
