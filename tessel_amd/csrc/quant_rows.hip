@@ -282,8 +282,8 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rmsnorm_q8_kernel(const u
 }
 
 // kv_write: keys rotated at pos, and values, into K and V [T, G, D] in f16 and into the cache in 4 bits.
-// The rotation is llm/kv_write's, x1 c - x2 s and x2 c + x1 s, in f64 (both products are exact there) and
-// rounded once, so that a key is the f16 nearest to its rotation.
+// The rotation is llm/kv_write's, x1 c - x2 s and x2 c + x1 s: one product rounded to f32, a multiply-add rounded to
+// f32, then f16 (rotate; rope_rotate's multiply-add may be rounded to f16 at once).
 //
 // A workgroup a token, D / 4 lanes a head: lane j holds channels 2j, 2j + 1 and their rotary
 // partners D/2 on, which are the bytes j and D/4 + j of the cache's row. Bound by its chain of loads
@@ -297,6 +297,12 @@ struct KvArgs {
     int T, W, NPOS, G, P;
     long NS;
 };
+
+TSL_DEV u16 rotate(float a, float c, float b, float s) {  // a c + b s
+    float y = __builtin_fmaf(a, c, b * s);
+    asm("" : "+v"(y));
+    return f2h(y);
+}
 
 template <int D>
 __global__ __launch_bounds__(512) void kv_write_q4_kernel(KvArgs a) {
@@ -334,9 +340,9 @@ __global__ __launch_bounds__(512) void kv_write_q4_kernel(KvArgs a) {
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                const double x1 = h2f(y[i]), x2 = h2f(y[2 + i]), ci = c[i], si = s[i];
-                y[i] = __builtin_bit_cast(u16, (half_t)(x1 * ci - x2 * si));
-                y[2 + i] = __builtin_bit_cast(u16, (half_t)(x2 * ci + x1 * si));
+                const float x1 = h2f(y[i]), x2 = h2f(y[2 + i]);
+                y[i] = rotate(x1, c[i], x2, -s[i]);
+                y[2 + i] = rotate(x2, c[i], x1, s[i]);
             }
         }
         float lo = INFINITY, hi = -INFINITY;
