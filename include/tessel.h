@@ -60,9 +60,11 @@ int tsl_fill_nan(uint64_t dst, size_t n);
  *                src/runtime.rs:202-236 Compiled::launch_raw) */
 
 /*
- * Kernel `name` of file `file` ("basic", "matmul", "attention", "llm"),
- * specialised for the array shapes given in parameter order: nshapes
- * arrays, array i has ranks[i] dimensions stored consecutively in dims.
+ * Kernel `name` of file `file` ("basic", "matmul", "attention", "llm"; not
+ * .tl files: "fused", the engine's fusions, and "quant", products, norms and
+ * rows in 8 bits and a paged cache in 4), specialised for the array shapes
+ * given in parameter order: nshapes arrays, array i has ranks[i] dimensions
+ * stored consecutively in dims.
  * meta_names/meta_values override the kernel's meta constants (an unknown
  * name is an error, src/ir.rs:1039-1043); warps is recorded in the key.
  * The same key "{file}/{name} {shapes:?} {meta:?} {warps}"
