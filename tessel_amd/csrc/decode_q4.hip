@@ -375,7 +375,8 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
     }
     // Of the head whose scores this lane takes (l16 % TPL): u's units (a scale of 0: nearly), and low's factor.
     const int head = (lane & 48) + l16 % TPL;
-    const float cs = __shfl(fmaxf(__builtin_ldexpf(__builtin_fabsf(a.c2), 24 - eq), 1e-37f), head);
+    const float unit = __builtin_ldexpf(__builtin_fabsf(a.c2), 24 - eq);
+    const float cs = __shfl(unit < 1e-37f ? 1e-37f : unit, head);  // (a NaN stays)
     const float qz = __shfl(__builtin_ldexpf(qsum, eq - 24) * (a.c2 < 0.0f ? -1.0f : 1.0f), head);
 
     const int ntiles = (len + TILE - 1) / TILE;

@@ -483,6 +483,15 @@ def test_decode_attention_scales_and_spoilt_queries(d, h, g):
     np.testing.assert_array_equal(got[~want], clean[~want])
 
 
+@pytest.mark.parametrize("d", [16, 32, 64, 128])
+def test_decode_attention_of_a_scale_that_is_no_number(d):
+    _say("decode_attention NaN scale", d)
+    for lens in ([70, 9], [1100, 20]):
+        case = _attention_case(np.random.default_rng(d), 2, 8, 2, d, 16, lens)
+        case[7] = float("nan")
+        assert np.isnan(_attend(*case)).all()
+
+
 @pytest.mark.parametrize("d,h,g", [(16, 4, 2), (32, 16, 1), (64, 8, 4), (128, 8, 1)])
 def test_decode_attention_small_and_large_values(d, h, g):
     # Values of 1e-5 to 6e4, alone and on neighbouring pages: probabilities keep their bits beside any step.
