@@ -637,7 +637,7 @@ int run_q4_d(const Q4Args& a, hipStream_t s) {
 
 }  // namespace
 
-int check_decode_q4(TslKernel& k) {
+int setup_decode_q4(TslKernel& k) {
     if (int r = check_cache_q4(k)) return r;
     const int64_t H = k.dim("H"), G = k.dim("G"), B = k.dim("B"), MP = k.dim("MP");
     if (H % G != 0) return tsl_fail(-2, "quant/decode_attention: H must be a multiple of G");
@@ -645,18 +645,10 @@ int check_decode_q4(TslKernel& k) {
     if (qpg != 1 && qpg != 2 && qpg != 4 && qpg != 8 && qpg != 16)
         return tsl_fail(-2, "quant/decode_attention: H / G must be 1, 2, 4, 8 or 16");
     if (k.dim("NP") == 0) return tsl_fail(-2, "quant/decode_attention: a pool of no pages");
-    if (MP > INT_MAX / k.dim("P") || B * H > (1 << 24) || B * G * nchunks(k) > (1 << 24))
-        return tsl_fail(-2, "quant/decode_attention: at most 2^31 - 1 tokens a table and 2^24 (sequence, head, chunk)s");
-    return 0;
-}
-
-int prepare_decode_q4(TslKernel& k) {
-    if (nchunks(k) > 1) {
-        const size_t bytes = (size_t)k.dim("B") * k.dim("H") * nchunks(k) * (2 + k.dim("D")) * sizeof(float);
-        if (bytes && tsl_hip_check(hipMalloc(&k.scratch, bytes), "quant/decode_attention scratch")) return -1;
-        k.scratch_bytes = bytes;
-    }
-    return 0;
+    // (a launch holds less than 2^32 work-items, 512 at most for each of these)
+    if (MP > INT_MAX / k.dim("P") || B * H > (1 << 22) || B * G * nchunks(k) > (1 << 22))
+        return tsl_fail(-2, "quant/decode_attention: at most 2^31 - 1 tokens a table and 2^22 (sequence, head, chunk)s");
+    return nchunks(k) > 1 ? tsl_scratch(k, (size_t)B * H * nchunks(k) * (2 + k.dim("D")) * sizeof(float)) : 0;
 }
 
 int launch_decode_q4(TslKernel& k, const uint64_t* args, hipStream_t s) {
@@ -675,6 +667,9 @@ int launch_decode_q4(TslKernel& k, const uint64_t* args, hipStream_t s) {
     a.wide = (int64_t)a.MP * a.P <= ONE_CHUNK;
     a.part = reinterpret_cast<float*>(k.scratch);
     if (a.B == 0) return 0;
+    // (slices of a pool by layer or page are aligned so: 16 tokens' codes are 128 bytes at least)
+    if ((args[1] | args[2]) % 16 || (args[3] | args[4]) % 16)
+        return tsl_fail(-2, "quant/decode_attention: Kc, Vc, Ks and Vs must be 16-byte aligned");
     switch (k.dim("D")) {
         case 16: return run_q4_d<16>(a, s);
         case 32: return run_q4_d<32>(a, s);

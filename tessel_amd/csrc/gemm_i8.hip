@@ -823,33 +823,22 @@ int run_gemm8(Gemm8 a, TslKernel& k, hipStream_t s) {
 }
 
 template <int EPI>
-int prepare_i8(TslKernel& k, const char* n) {
-    Gemm8 a{};
-    a.M = (int)k.dim("M"), a.N = (int)k.dim(n), a.K = (int)k.dim("K");
-    if (const size_t bytes = packed_bytes<EPI>(a)) {
-        if (tsl_hip_check(hipMalloc(&k.scratch, bytes), ("quant/" + k.name + " scratch").c_str())) return -1;
-        k.scratch_bytes = bytes;
-    }
-    return 0;
-}
-
-int check_i8(const TslKernel& k, const char* n) {
+int setup_i8(TslKernel& k, const char* n) {
     if (k.dim("K") > 131071)
         return tsl_fail(-2, "quant/" + k.name + ": K = " + std::to_string(k.dim("K")) + " exceeds 131071 (sums of 8-bit products in 32 bits)");
     if (k.dim("M") > (1 << 24) || k.dim(n) > (1 << 24))
         return tsl_fail(-2, "quant/" + k.name + ": at most 2^24 rows and columns");
-    // (a launch holds 2^32 work-items; 512 of them make 64 x 32 outputs at least)
-    if ((k.dim("M") + 63) * (k.dim(n) + 31) > (1LL << 34)) return tsl_fail(-2, "quant/" + k.name + ": at most 2^34 outputs");
-    return 0;
+    // (a launch holds less than 2^32 work-items; 512 of them make 64 x 32 outputs at least)
+    if ((k.dim("M") + 63) * (k.dim(n) + 31) >= (1LL << 34)) return tsl_fail(-2, "quant/" + k.name + ": at most 2^34 outputs");
+    Gemm8 a{};
+    a.M = (int)k.dim("M"), a.N = (int)k.dim(n), a.K = (int)k.dim("K");
+    return tsl_scratch(k, packed_bytes<EPI>(a));
 }
 
 }  // namespace
 
-int check_linear_q8(TslKernel& k) { return check_i8(k, "N"); }
-int check_gate_up_q8(TslKernel& k) { return check_i8(k, "F"); }
-
-int prepare_linear_q8(TslKernel& k) { return prepare_i8<Q_LINEAR>(k, "N"); }
-int prepare_gate_up_q8(TslKernel& k) { return prepare_i8<Q_SWIGLU>(k, "F"); }
+int setup_linear_q8(TslKernel& k) { return setup_i8<Q_LINEAR>(k, "N"); }
+int setup_gate_up_q8(TslKernel& k) { return setup_i8<Q_SWIGLU>(k, "F"); }
 
 int launch_linear_q8(TslKernel& k, const uint64_t* a, hipStream_t s) {
     return run_gemm8<Q_LINEAR>({P<int8_t>(a[0]), P<int8_t>(a[2]), nullptr, P<float>(a[1]), P<float>(a[3]), nullptr,

@@ -449,8 +449,8 @@ int run_rmsnorm_q8(TslKernel& k, const u16* X, const uint64_t* a, hipStream_t s)
 
 }  // namespace
 
-int check_quantize(TslKernel& k) { return check_rows(k, "M", "K"); }
-int check_rmsnorm_q8(TslKernel& k) {
+int setup_quantize(TslKernel& k) { return check_rows(k, "M", "K"); }
+int setup_rmsnorm_q8(TslKernel& k) {
     if (k.dim("Dm") == 0) return tsl_fail(-2, "quant/" + k.name + ": rows of 0 columns");
     return check_rows(k, "T", "Dm");
 }
@@ -485,12 +485,12 @@ int check_cache_q4(const TslKernel& k) {
     return 0;
 }
 
-int check_kv_write_q4(TslKernel& k) {
+int setup_kv_write_q4(TslKernel& k) {
     if (int r = check_cache_q4(k)) return r;
     if (k.dim("W") < 2 * k.dim("G") * k.dim("D"))
         return tsl_fail(-2, "quant/kv_write: rows of W = " + std::to_string(k.dim("W")) + " hold no 2 G D keys and values");
-    if (k.dim("T") > (1 << 23) || k.dim("W") > INT_MAX || k.dim("NPOS") > INT_MAX)
-        return tsl_fail(-2, "quant/kv_write: at most 2^23 tokens, and sizes below 2^31");
+    if (k.dim("T") >= (1 << 23) || k.dim("W") > INT_MAX || k.dim("NPOS") > INT_MAX)
+        return tsl_fail(-2, "quant/kv_write: tokens below 2^23 and sizes below 2^31");
     return 0;
 }
 

@@ -64,15 +64,20 @@ int launch_kv_write_q4(TslKernel&, const uint64_t*, hipStream_t);
 int launch_linear_q8(TslKernel&, const uint64_t*, hipStream_t);
 int launch_gate_up_q8(TslKernel&, const uint64_t*, hipStream_t);
 int launch_decode_q4(TslKernel&, const uint64_t*, hipStream_t);
-int check_quantize(TslKernel&);
-int check_rmsnorm_q8(TslKernel&);
-int check_kv_write_q4(TslKernel&);
-int check_linear_q8(TslKernel&);
-int check_gate_up_q8(TslKernel&);
-int check_decode_q4(TslKernel&);
-int prepare_decode_q4(TslKernel&);
-int prepare_linear_q8(TslKernel&);
-int prepare_gate_up_q8(TslKernel&);
+int setup_quantize(TslKernel&);
+int setup_rmsnorm_q8(TslKernel&);
+int setup_kv_write_q4(TslKernel&);
+int setup_linear_q8(TslKernel&);
+int setup_gate_up_q8(TslKernel&);
+int setup_decode_q4(TslKernel&);
+
+int tsl_scratch(TslKernel& k, size_t bytes) {
+    if (!bytes) return 0;
+    if (int r = tsl_open()) return r;
+    if (int r = tsl_hip_check(hipMalloc(&k.scratch, bytes), (k.file + "/" + k.name + " scratch").c_str())) return r;
+    k.scratch_bytes = bytes;
+    return 0;
+}
 
 // Compute units of the current device (cached; 256 if the query fails).
 int num_cus() {
@@ -109,7 +114,7 @@ struct KernelDef {
     const char* pow2;  // dimensions the body slices in full (tile sizes: powers of two)
     tsl_launcher launch;
     tsl_preparer prepare;
-    tsl_preparer check = nullptr;  // sizes the kernel refuses (before any device is touched)
+    tsl_preparer setup = nullptr;  // refuses sizes, and takes scratch (tsl_scratch) where the sizes need some
     std::vector<Param> params;
     std::vector<std::pair<std::string, int64_t>> meta_defaults;
 };
@@ -200,27 +205,27 @@ std::vector<KernelDef> g_defs = {
     // Rows in 8 bits are codes and one f32 step a row: value = S Q. quantize
     // serves weights (rows are channels) as it serves activations; the norms'
     // outputs are quantised unrounded, add_rmsnorm after R += X.
-    {"quant", "quantize", "X: f16[M, K], Q: i8[M, K], S: f32[M]", "", "", launch_quantize, nullptr, check_quantize},
+    {"quant", "quantize", "X: f16[M, K], Q: i8[M, K], S: f32[M]", "", "", launch_quantize, nullptr, setup_quantize},
     {"quant", "rmsnorm", "R: f32[T, Dm], W: f16[Dm], Q: i8[T, Dm], S: f32[T], eps: f32", "", "", launch_rmsnorm_q8,
-     nullptr, check_rmsnorm_q8},
+     nullptr, setup_rmsnorm_q8},
     {"quant", "add_rmsnorm", "X: f16[T, Dm], R: f32[T, Dm], W: f16[Dm], Q: i8[T, Dm], S: f32[T], eps: f32", "", "",
-     launch_add_rmsnorm_q8, nullptr, check_rmsnorm_q8},
+     launch_add_rmsnorm_q8, nullptr, setup_rmsnorm_q8},
     // llm/linear and llm/gate_up of such rows: X SX, W SW.
     {"quant", "linear", "X: i8[M, K], SX: f32[M], W: i8[N, K], SW: f32[N], Y: f16[M, N]", "", "", launch_linear_q8,
-     prepare_linear_q8, check_linear_q8},
+     nullptr, setup_linear_q8},
     {"quant", "gate_up",
      "X: i8[M, K], SX: f32[M], Wg: i8[F, K], SG: f32[F], Wu: i8[F, K], SU: f32[F], Y: f16[M, F]", "", "",
-     launch_gate_up_q8, prepare_gate_up_q8, check_gate_up_q8},
+     launch_gate_up_q8, nullptr, setup_gate_up_q8},
     // llm/kv_write and llm/decode_attention with the cache in 4 bits: codes two
     // a byte, and (lowest value, step) of each token and kv head.
     {"quant", "kv_write",
      "QKV: f16[T, W], pos: i32[T], slot: i32[T], C: f32[NPOS, D2], S: f32[NPOS, D2], Kc: u8[NP, G, P, D2], "
      "Vc: u8[NP, G, PB, D2, 16], Ks: f16[NP, G, P, 2], Vs: f16[NP, G, P, 2], K: f16[T, G, D], V: f16[T, G, D]",
-     "", "P D", launch_kv_write_q4, nullptr, check_kv_write_q4},
+     "", "P D", launch_kv_write_q4, nullptr, setup_kv_write_q4},
     {"quant", "decode_attention",
      "Q: f16[B, H, D], Kc: u8[NP, G, P, D2], Vc: u8[NP, G, PB, D2, 16], Ks: f16[NP, G, P, 2], Vs: f16[NP, G, P, 2], "
      "table: i32[B, MP], lens: i32[B], O: f16[B, H, D], scale: f32",
-     "", "P D", launch_decode_q4, prepare_decode_q4, check_decode_q4},
+     "", "P D", launch_decode_q4, nullptr, setup_decode_q4},
 };
 
 std::string trim(const std::string& s) {
@@ -521,8 +526,8 @@ int tsl_kernel(const char* file, const char* name, int nshapes, const int* ranks
             if (!pow2(k->dim(dn.c_str())))
                 return bad("tile dimensions must be powers of two, got " + dn + " = " + std::to_string(k->dim(dn.c_str())));
     }
-    if (def->check) {
-        if (int r = def->check(*k)) {
+    if (def->setup) {
+        if (int r = def->setup(*k)) {
             delete k;
             return r;
         }

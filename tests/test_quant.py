@@ -53,7 +53,10 @@ def _write(t=3, w=768, g=2, d=64, p=16, **kw):
     ("decode_attention", _decode(d2=16), "D2 must be D / 2"),
     ("decode_attention", _decode(p=8, pb=1), "multiple of 16 tokens"),
     ("decode_attention", _decode(mp=2 ** 28), "tokens a table"),
-    ("decode_attention", _decode(b=2 ** 23), "2\\^24"),
+    ("decode_attention", _decode(b=2 ** 23), "2\\^22"),
+    ("decode_attention", _decode(b=2 ** 19 + 1), "2\\^22"),
+    ("linear", [[2 ** 20 - 63, 64], [2 ** 20 - 63], [2 ** 14 - 31, 64], [2 ** 14 - 31], [2 ** 20 - 63, 2 ** 14 - 31]], "at most 2\\^34"),
+    ("kv_write", _write(t=2 ** 23), "below 2\\^23"),
     ("decode_attention", [x[:0] + [0] + x[1:] if len(x) > 2 and x[0] == 4 else x for x in _decode()], "pool of no pages"),
     ("decode_attention", [[3, 8, 64]], "no shape given"),
     ("linear_residual", [], "no kernel linear_residual"),

@@ -483,6 +483,18 @@ def test_decode_attention_scales_and_spoilt_queries(d, h, g):
     np.testing.assert_array_equal(got[~want], clean[~want])
 
 
+def test_decode_attention_refuses_a_pool_off_its_alignment():
+    kern = T.kernel("quant", "decode_attention", [[1, 4, 64], [2, 2, 16, 32], [2, 2, 1, 32, 16], [2, 2, 16, 2], [2, 2, 16, 2],
+                                                  [1, 2], [1], [1, 4, 64]])
+    bufs = [T.alloc(n + 64) for n in (512, 2048, 2048, 256, 256, 8, 4, 512)]
+    for i in (1, 2, 3, 4):
+        at = [T.Buf(b.ptr + (8 if j == i else 0), b.bytes - 64) for j, b in enumerate(bufs)]
+        with pytest.raises(T.TesselError, match="16-byte aligned"):
+            T.launch(kern, at + [T.F32(0.125)])
+    for b in bufs:
+        T.free(b)
+
+
 @pytest.mark.parametrize("d", [16, 32, 64, 128])
 def test_decode_attention_of_a_scale_that_is_no_number(d):
     _say("decode_attention NaN scale", d)
