@@ -21,7 +21,6 @@ constexpr int NUM_XCD = 8;
 enum Epi8 { Q_LINEAR, Q_SWIGLU };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef u32x4 u32x4b __attribute__((aligned(1)));
 
 struct Gemm8 {
     const int8_t *X, *W, *W2;        // W2: gate_up's Wu
@@ -57,158 +56,48 @@ TSL_DEV void tile_of(int bid, int nwg, int tiles_m, int tiles_n, int G, int& tm,
     tn = (pid % width) / rows;
 }
 
-// 16 k of a row from k (a multiple of 16) on, zeros past K: one load at byte alignment. A chunk that crosses the
-// row's end is the row's last 16 bytes, shifted, so that nothing past a row is read.
-TSL_DEV u32x4 row16(const int8_t* row, int k, int K) {
-    if (k + 16 <= K) return (u32x4) * reinterpret_cast<const u32x4b*>(row + k);
-    u32x4 v = {0, 0, 0, 0};
-    if (k >= K) return v;
-    if (K >= 16) {
-        typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
-        u64x2 q = __builtin_bit_cast(u64x2, (u32x4) * reinterpret_cast<const u32x4b*>(row + K - 16));
-        const int drop = 8 * (k + 16 - K);  // 8 .. 120 bits
-        if (drop >= 64) q = u64x2{q[1], 0};
-        const int d = drop & 63;
-        if (d) q = u64x2{q[0] >> d | q[1] << (64 - d), q[1] >> d};
-        return __builtin_bit_cast(u32x4, q);
-    }
+// 16 k of a row of any alignment from k (a multiple of 16) on, zeros past K: the aligned words that hold them, and
+// their shift in a second step (value), so that the loads of later steps can be under way. The fifth
+// word is the next lane's first where that lane has the row's next 16 k (lone: it has not), else loaded. A chunk past
+// the row's end loads the row's last 16 bytes, so that no word is read that holds no byte of the row.
+// (16 bytes at byte alignment take 2 us longer than at 4 in 777 x 1008 x 1155 products, a loaded fifth word of every
+// chunk 1.)
+struct Row16 {
+    u32x4 v;
+    uint32_t e = 0;
+    TSL_DEV void load(const int8_t* row, int k, int K, bool lone) {
+        typedef u32x4 u32x4w __attribute__((aligned(4)));
+        if (K >= 16) {
+            const int8_t* p = row + min(k, K - 16);
+            const uint32_t s = (uint32_t)(uintptr_t)p & 3;
+            v = *reinterpret_cast<const u32x4w*>(p - s);
+            if (s && (lone || k + 32 > K)) e = *reinterpret_cast<const uint32_t*>(p - s + 16);
+        } else {
+            v = u32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int e = 0; e < 15; e++)
-        if (k + e < K) v[e >> 2] |= (uint32_t)(uint8_t)row[k + e] << (8 * (e & 3));
-    return v;
-}
-
-// Any K and alignment: 16-byte loads at byte alignment into registers, a step ahead, then LDS.
-// 64 x 64 products a workgroup; KG groups of 4 wavefronts take steps g, g + KG, .. of 128 k
-// through two stages of their own, and their sums are added through LDS at the end (4 groups
-// where the tiles make one round on the CUs, else 2: 33 x 2049 x 4095 16.5 / 18.5 us).
-// gate_up's tile holds, for each wavefront column, WN / 2 rows of Wg and their partners of
-// Wu, so a lane has both sums of an output.
-//
-// Bound by the loads, which straddle lines: 777 x 1155 x 1001 9.5 us (12.5 with one group and each
-// step's loads waited for), 4001 x 4001 x 1001 95.
-template <int EPI, int KG>
-__global__ __launch_bounds__(256 * KG) void gemm_i8_any(Gemm8 a) {
-    constexpr bool DUAL = EPI == Q_SWIGLU;
-    constexpr int BM = 64, BN = 64;
-    constexpr int BK = 128, KC = BK / 16;                   // bytes and 16-byte chunks of a tile row
-    constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16;
-    constexpr int CA = BM * KC / 256, CB = BN * KC / 256;   // chunks a thread
-    constexpr int OUT = DUAL ? BN / 2 : BN;                 // columns of Y a tile
-    constexpr int STAGE = (BM + BN) * KC;
-    __shared__ __attribute__((aligned(16))) u32x4 lds[KG * 2 * STAGE];
-    TSL_POISON(lds);
-    auto sw = [](int r) { return (r >> 1) & 7; };
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = threadIdx.x & 255;
-    const int kg = wave >> 2, w4 = wave & 3;
-    const int wm0 = (w4 >> 1) * WM, wn0 = (w4 & 1) * WN;
-    int tm, tn;
-    tile_of(blockIdx.x, gridDim.x, (a.M + BM - 1) / BM, (a.N + OUT - 1) / OUT, 8, tm, tn);
-    const int m0 = tm * BM, n0 = tn * OUT, K = a.K;
-    u32x4* ring = lds + kg * 2 * STAGE;
-    // Tile row r of B: the row of W (or Wu) it holds.
-    auto brow = [&](int r) -> const int8_t* {
-        if constexpr (!DUAL) return a.W + (size_t)min(n0 + r, a.N - 1) * K;
-        const int j = r % WN, n = n0 + (r / WN) * (WN / 2) + j % (WN / 2);
-        return (j < WN / 2 ? a.W : a.W2) + (size_t)min(n, a.N - 1) * K;
-    };
-    const int8_t *pa[CA], *pb[CB];
-    const int c16 = 16 * (t % KC);  // this thread's chunk of every row it loads
-#pragma unroll
-    for (int i = 0; i < CA; i++) pa[i] = a.X + (size_t)min(m0 + (i * 256 + t) / KC, a.M - 1) * K;
-#pragma unroll
-    for (int i = 0; i < CB; i++) pb[i] = brow((i * 256 + t) / KC);
-    i32x4 acc[TM][TN];
-#pragma unroll
-    for (int i = 0; i < TM; i++)
-#pragma unroll
-        for (int j = 0; j < TN; j++) acc[i][j] = i32x4{};
-    const int l16 = lane & 15, g16 = lane >> 4;
-    const int rounds = ((K + BK - 1) / BK + KG - 1) / KG;  // (a group past the end multiplies zeros)
-    u32x4 ra[CA], rb[CB];
-    auto gload = [&](int round) {
-        const int k = (round * KG + kg) * BK + c16;
-#pragma unroll
-        for (int i = 0; i < CA; i++) ra[i] = row16(pa[i], k, K);
-#pragma unroll
-        for (int i = 0; i < CB; i++) rb[i] = row16(pb[i], k, K);
-    };
-    auto sstore = [&](int stage) {
-        u32x4* s = ring + stage * STAGE;
-#pragma unroll
-        for (int i = 0; i < CA; i++) {
-            const int r = (i * 256 + t) / KC;
-            s[r * KC + ((t % KC) ^ sw(r))] = ra[i];
+            for (int i = 0; i < 15; i++)
+                if (k + i < K) v[i >> 2] |= (uint32_t)(uint8_t)row[k + i] << (8 * (i & 3));
         }
-#pragma unroll
-        for (int i = 0; i < CB; i++) {
-            const int r = (i * 256 + t) / KC;
-            s[BM * KC + r * KC + ((t % KC) ^ sw(r))] = rb[i];
+    }
+    TSL_DEV u32x4 value(const int8_t* row, int k, int K, bool lone) const {
+        if (K < 16) return v;
+        const uint32_t next = __builtin_amdgcn_mov_dpp((int)v[0], 0x101, 0xf, 0xf, true);  // row_shl:1
+        const uint32_t s = (uint32_t)(uintptr_t)(row + min(k, K - 16)) & 3, x = lone || k + 32 > K ? e : next;
+        u32x4 w = {__builtin_amdgcn_alignbyte(v[1], v[0], s), __builtin_amdgcn_alignbyte(v[2], v[1], s),
+                   __builtin_amdgcn_alignbyte(v[3], v[2], s), __builtin_amdgcn_alignbyte(x, v[3], s)};
+        // (No 64-bit shifts: one by an amount that lay in the wavefront's last VGPR gave random results.)
+        const int drop = k + 16 - K;  // bytes past K
+        if (drop > 0) {
+            const bool d8 = drop & 8, d4 = drop & 4;
+            const uint32_t a = d8 ? w[2] : w[0], b = d8 ? w[3] : w[1], c = d8 ? 0 : w[2], d = d8 ? 0 : w[3];
+            const uint32_t p = d4 ? b : a, q = d4 ? c : b, r = d4 ? d : c, t = d4 ? 0 : d;
+            w = u32x4{__builtin_amdgcn_alignbyte(q, p, drop), __builtin_amdgcn_alignbyte(r, q, drop),
+                      __builtin_amdgcn_alignbyte(t, r, drop), __builtin_amdgcn_alignbyte(0, t, drop)};
+            if (drop >= 16) w = u32x4{0, 0, 0, 0};
         }
-    };
-    if (rounds > 0) {
-        gload(0);
-        sstore(0);
+        return w;
     }
-    for (int q = 0; q < rounds; q++) {
-        __syncthreads();  // stage q is written, and every read of the other is done
-        if (q + 1 < rounds) gload(q + 1);
-        const u32x4* s = ring + (q & 1) * STAGE;
-#pragma unroll
-        for (int st = 0; st < BK / 64; st++) {
-            i32x4 av[TM], bv[TN];
-#pragma unroll
-            for (int i = 0; i < TM; i++) {
-                const int r = wm0 + i * 16 + l16;
-                av[i] = __builtin_bit_cast(i32x4, s[r * KC + ((4 * st + g16) ^ sw(r))]);
-            }
-#pragma unroll
-            for (int j = 0; j < TN; j++) {
-                const int r = wn0 + j * 16 + l16;
-                bv[j] = __builtin_bit_cast(i32x4, s[BM * KC + r * KC + ((4 * st + g16) ^ sw(r))]);
-            }
-#pragma unroll
-            for (int i = 0; i < TM; i++)
-#pragma unroll
-                for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(av[i], bv[j], acc[i][j], 0, 0, 0);
-        }
-        if (q + 1 < rounds) sstore((q + 1) & 1);
-    }
-    __syncthreads();
-    i32x4* red = reinterpret_cast<i32x4*>(lds);  // [KG - 1][4 wavefronts][TM TN][64]
-    if (kg > 0)
-#pragma unroll
-        for (int i = 0; i < TM; i++)
-#pragma unroll
-            for (int j = 0; j < TN; j++) red[(((kg - 1) * 4 + w4) * TM * TN + i * TN + j) * 64 + lane] = acc[i][j];
-    __syncthreads();
-    if (kg > 0) return;
-#pragma unroll
-    for (int g = 0; g < KG - 1; g++)
-#pragma unroll
-        for (int i = 0; i < TM; i++)
-#pragma unroll
-            for (int j = 0; j < TN; j++) acc[i][j] += red[((g * 4 + w4) * TM * TN + i * TN + j) * 64 + lane];
-    // Lane l of a 16 x 16 tile: column l % 16, rows 4 (l / 16) + r.
-    constexpr int TNO = DUAL ? TN / 2 : TN;
-#pragma unroll
-    for (int j = 0; j < TNO; j++) {
-        const int n = n0 + (DUAL ? wn0 / 2 : wn0) + j * 16 + l16;
-        if (n >= a.N) continue;
-        const float sw1 = a.SW[n], sw2 = DUAL ? a.SW2[n] : 0.0f;
-#pragma unroll
-        for (int i = 0; i < TM; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int m = m0 + wm0 + i * 16 + 4 * g16 + r;
-                if (m >= a.M) continue;
-                const float sx = a.SX[m];
-                float v = scaled(acc[i][j][r], sx, sw1);
-                if constexpr (DUAL) v = silu_mul(v, scaled(acc[i][j + TNO][r], sx, sw2));
-                a.Y[(size_t)m * a.N + n] = f2h(v);
-            }
-    }
-}
+};
 
 // ---------------------------------------------------------------- aligned rows
 // K % 16 == 0 and 16-byte aligned operands: tiles go from global memory into LDS by
@@ -321,6 +210,126 @@ template <bool DUAL, int WN>
 TSL_DEV int w_row(int r) { return DUAL ? (r / WN) * (WN / 2) + r % (WN / 2) : r; }
 template <bool DUAL, int WN>
 TSL_DEV bool w_up(int r) { return DUAL && r % WN >= WN / 2; }
+
+// Any K and alignment: 16 bytes a lane into registers (Row16), two steps ahead, then LDS.
+// 64 x 64 products a workgroup, operands and outputs laid out as the aligned tiles' are; KG groups of 4 wavefronts take
+// steps g, g + KG, .. of 128 k through two stages of their own, and their sums are added through LDS at the end (4
+// groups where the tiles make one round on the CUs, else 2).
+//
+// Bound by latency (777 x 1155 x 1001 7.1 us; with loads one step ahead, a load at byte alignment a chunk and
+// outputs stored one at a time 9.4), then by the loads, which straddle lines (4001 x 4001 x 1001 71).
+template <int EPI, int KG>
+__global__ __launch_bounds__(256 * KG) void gemm_i8_any(Gemm8 a) {
+    constexpr bool DUAL = EPI == Q_SWIGLU;
+    constexpr int BM = 64, BN = 64;
+    constexpr int BK = 128, KC = BK / 16;                   // bytes and 16-byte chunks of a tile row
+    constexpr int WM = BM / 2, WN = BN / 2, TM = WM / 16, TN = WN / 16, TNO = DUAL ? TN / 2 : TN;
+    constexpr int CA = BM * KC / 256, CB = BN * KC / 256;   // chunks a thread
+    constexpr int OUT = DUAL ? BN / 2 : BN;                 // columns of Y a tile
+    constexpr int STAGE = (BM + BN) * KC;
+    __shared__ __attribute__((aligned(16))) u32x4 lds[KG * 2 * STAGE];
+    TSL_POISON(lds);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = threadIdx.x & 255;
+    const int kg = wave >> 2, w4 = wave & 3;
+    const int wm0 = (w4 >> 1) * WM, wn0 = (w4 & 1) * WN;
+    int tm, tn;
+    tile_of(blockIdx.x, gridDim.x, (a.M + BM - 1) / BM, (a.N + OUT - 1) / OUT, 8, tm, tn);
+    const int m0 = tm * BM, n0 = tn * OUT, K = a.K;
+    u32x4* ring = lds + kg * 2 * STAGE;
+    const int8_t *pa[CA], *pb[CB];
+    const int c16 = 16 * (t % KC);  // this thread's chunk of every row it loads
+#pragma unroll
+    for (int i = 0; i < CA; i++) pa[i] = a.X + (size_t)min(m0 + (i * 256 + t) / KC, a.M - 1) * K;
+#pragma unroll
+    for (int i = 0; i < CB; i++) {
+        const int r = (i * 256 + t) / KC;
+        pb[i] = (w_up<DUAL, WN>(r) ? a.W2 : a.W) + (size_t)min(n0 + w_row<DUAL, WN>(r), a.N - 1) * K;
+    }
+    i32x4 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; i++)
+#pragma unroll
+        for (int j = 0; j < TN; j++) acc[i][j] = i32x4{};
+    const int l16 = lane & 15, g16 = lane >> 4;
+    const int xr = wm0 + l16, wr = wn0 + 4 * TNO * (l16 >> 2) + (l16 & 3);  // tile 0's operand rows
+    const int rounds = ((K + BK - 1) / BK + KG - 1) / KG;  // (a group past the end multiplies zeros)
+    struct Chunks {
+        Row16 a[CA], b[CB];
+    };
+    const bool lone = t % KC == KC - 1;
+    auto gload = [&](int round, Chunks& x) {
+        const int k = (round * KG + kg) * BK + c16;
+#pragma unroll
+        for (int i = 0; i < CA; i++) x.a[i].load(pa[i], k, K, lone);
+#pragma unroll
+        for (int i = 0; i < CB; i++) x.b[i].load(pb[i], k, K, lone);
+    };
+    auto sstore = [&](int round, const Chunks& x) {
+        u32x4* s = ring + (round & 1) * STAGE;
+        const int k = (round * KG + kg) * BK + c16;
+#pragma unroll
+        for (int i = 0; i < CA; i++) {
+            const int r = (i * 256 + t) / KC;
+            s[r * KC + ((t % KC) ^ swx(r))] = x.a[i].value(pa[i], k, K, lone);
+        }
+#pragma unroll
+        for (int i = 0; i < CB; i++) {
+            const int r = (i * 256 + t) / KC;
+            s[BM * KC + r * KC + ((t % KC) ^ sww<TNO>(r))] = x.b[i].value(pb[i], k, K, lone);
+        }
+    };
+    // Round q: its stage is written and the other's reads are done; x, the next round's chunks, go to that one, and
+    // the round after that is loaded into them.
+    auto round = [&](int q, Chunks& x) {
+        __syncthreads();
+        const u32x4* s = ring + (q & 1) * STAGE;
+#pragma unroll
+        for (int st = 0; st < BK / 64; st++) {
+            i32x4 xv[TM], wv[TN];
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+                xv[i] = __builtin_bit_cast(i32x4, s[(xr + 16 * i) * KC + ((4 * st + g16) ^ swx(xr))]);
+#pragma unroll
+            for (int j = 0; j < TN; j++) {
+                const int r = wr + (j / TNO) * (WN / 2) + 4 * (j % TNO);
+                wv[j] = __builtin_bit_cast(i32x4, s[BM * KC + r * KC + ((4 * st + g16) ^ sww<TNO>(r))]);
+            }
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+#pragma unroll
+                for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[j], xv[i], acc[i][j], 0, 0, 0);
+        }
+        if (q + 1 < rounds) sstore(q + 1, x);
+        if (q + 3 < rounds) gload(q + 3, x);
+    };
+    if (rounds > 0) {
+        Chunks x, y;
+        gload(0, x);
+        if (rounds > 1) gload(1, y);
+        sstore(0, x);
+        if (rounds > 2) gload(2, x);
+        for (int q = 0; q < rounds; q += 2) {
+            round(q, y);
+            if (q + 1 < rounds) round(q + 1, x);
+        }
+    }
+    __syncthreads();
+    i32x4* red = reinterpret_cast<i32x4*>(lds);  // [KG - 1][4 wavefronts][TM TN][64]
+    if (kg > 0)
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int j = 0; j < TN; j++) red[(((kg - 1) * 4 + w4) * TM * TN + i * TN + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    if (kg > 0) return;
+#pragma unroll
+    for (int g = 0; g < KG - 1; g++)
+#pragma unroll
+        for (int i = 0; i < TM; i++)
+#pragma unroll
+            for (int j = 0; j < TN; j++) acc[i][j] += red[((g * 4 + w4) * TM * TN + i * TN + j) * 64 + lane];
+    store_tiles<EPI, TM, TN>(a, m0 + wm0, n0 + (DUAL ? wn0 / 2 : wn0), lane, acc);
+}
 
 // BM x BN tiles, WGM x WGN wavefronts, NS stages of 128 k in a ring. KG groups of wavefronts with a
 // ring each take steps g, g + KG, ..; their sums are added through LDS at the end.
@@ -738,7 +747,12 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(Gemm8 a, int8_t* __restr
         }
         const int8_t* row = from + (size_t)r * a.K;
         int8_t* to = out + (size_t)i * Kp;
-        for (int k = 16 * (threadIdx.x & 63); k < Kp; k += 1024) *reinterpret_cast<u32x4*>(to + k) = row16(row, k, a.K);
+        const bool lone = (threadIdx.x & 15) == 15;
+        for (int k = 16 * (threadIdx.x & 63); k < Kp; k += 1024) {
+            Row16 x;
+            x.load(row, k, a.K, lone);
+            *reinterpret_cast<u32x4*>(to + k) = x.value(row, k, a.K, lone);
+        }
     }
 }
 
@@ -787,9 +801,10 @@ int run_aligned(const Gemm8& a, hipStream_t s) {
     }
 }
 
-// Whether rows of K no multiple of 16 are copied first (into the handle's scratch): gemm_i8_any takes 4 us and, a
-// step, 0.39 us or its share of 0.7 us a round of the CUs; the copy 4 us and its bytes at 3 TB/s, then the
-// aligned forms (us, any / copied: 4001 x 4001 x 1001 95 / 38, 33 x 2049 x 4095 16.5 / 12.0, 777 x 1155 x 1001 9.5 / 9.8).
+// Whether rows of K no multiple of 16 are copied first (into the handle's scratch): gemm_i8_any takes 3.5 us and, a
+// step, 0.36 us or its share of 0.55 us a round of the CUs; the copy 3 us and its bytes at 3 TB/s, then the
+// aligned forms (us, any / copied: 4001 x 4001 x 1001 71 / 37, 1500 x 2100 x 2001 29.7 / 19.7, 100 x 500 x 9001 27.9
+// / 22.1, 777 x 1155 x 1001 7.1 / 9.4, 513 x 3001 x 777 9.9 / 13.2, 1 x 9001 x 4001 17.1 / 22.3).
 template <int EPI>
 long any_tiles(const Gemm8& a) {
     constexpr int OUT = EPI == Q_SWIGLU ? 32 : 64;
@@ -798,10 +813,10 @@ long any_tiles(const Gemm8& a) {
 template <int EPI>
 size_t packed_bytes(Gemm8 a) {
     if (a.K % 16 == 0 || a.M == 0 || a.N == 0) return 0;
-    const double steps = (a.K + 127) / 128, any = 4.0 + steps * std::max(0.39, 0.7 * any_tiles<EPI>(a) / num_cus());
+    const double steps = (a.K + 127) / 128, any = 3.5 + steps * std::max(0.36, 0.55 * any_tiles<EPI>(a) / num_cus());
     a.K = (a.K + 127) / 128 * 128;
     const size_t bytes = ((size_t)a.M + (EPI == Q_SWIGLU ? 2 : 1) * (size_t)a.N) * a.K;
-    return 4.0 + bytes * 2 / 3e6 + plan_aligned<EPI>(a).us < any ? bytes : 0;
+    return 3.0 + bytes * 2 / 3e6 + plan_aligned<EPI>(a).us < any ? bytes : 0;
 }
 
 template <int EPI>

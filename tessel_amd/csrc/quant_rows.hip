@@ -384,15 +384,10 @@ __global__ __launch_bounds__(512) void kv_write_q4_kernel(KvArgs a) {
         if (!keep) continue;
         const long head = page * a.G + g;
         const uint8_t b0 = (uint8_t)(n[0] | n[1] << 4), b1 = (uint8_t)(n[2] | n[3] << 4);
-        if (val) {
-            uint8_t* c = a.Vc + (head * (a.P / 16) + off / 16) * (D2 * 16) + off % 16;
-            c[lane * 16] = b0;
-            c[(D2 / 2 + lane) * 16] = b1;
-        } else {
-            uint8_t* c = a.Kc + (head * a.P + off) * D2;
-            c[lane] = b0;
-            c[D2 / 2 + lane] = b1;
-        }
+        // (token off: K's row of D2 bytes; V's byte off % 16 of every 16 in its block)
+        uint8_t* c = (val ? a.Vc : a.Kc) + (head * a.P + (val ? off & ~15 : off)) * D2 + (val ? off & 15 : 0);
+        c[lane * (val ? 16 : 1)] = b0;
+        c[(D2 / 2 + lane) * (val ? 16 : 1)] = b1;
         if (lane == 0) {
             u16* s = (val ? a.Vs : a.Ks) + (head * a.P + off) * 2;
             s[0] = bad ? (u16)0x7e00 : f2h(lo);
