@@ -228,6 +228,64 @@ def test_linear_at_any_alignment(m, n, k):
             T.free(b)
 
 
+@pytest.mark.parametrize("m,f,k,launches", [(70, 300, 1001, 1), (9, 40, 2048, 1), (1000, 1155, 1001, 2), (40, 33, 13, 1)])
+def test_gate_up_at_any_alignment(m, f, k, launches):
+    # Operands that begin at odd addresses, each at another, give the bits of aligned ones; with one column of Wu spoilt by
+    # its step, and a graph that says whether rows are copied first.
+    _say("gate_up unaligned", m, f, k)
+    rng = np.random.default_rng(m + f + k)
+    _check_gate_up(rng, m, f, k)
+    (x, sx), (wg, sg), (wu, su) = _rows(rng, m, k), _rows(rng, f, k), _rows(rng, f, k)
+    su[f // 2] = np.nan
+    want = run("gate_up", [x, sx, wg, sg, wu, su, np.full((m, f), 7, np.float16)], outputs=[6])[6]
+    assert np.isnan(want[:, f // 2]).all() and np.isnan(want).sum() == m
+    kern = T.kernel("quant", "gate_up", [x.shape, sx.shape, wg.shape, sg.shape, wu.shape, su.shape, (m, f)])
+    for offs in ((1, 2, 3), (15, 0, 8)):
+        bufs = [T.alloc(v.nbytes + 32) for v in (x, wg, wu)]
+        bsx, bsg, bsu, by = T.tensor(sx), T.tensor(sg), T.tensor(su), T.alloc(2 * m * f + 64)
+        for b, v, o in zip(bufs, (x, wg, wu), offs):
+            T.write(b, o, v)
+        bx, bg, bu = (T.Buf(b.ptr + o, v.nbytes) for b, v, o in zip(bufs, (x, wg, wu), offs))
+        T.capture_begin()
+        T.launch(kern, [bx, bsx, bg, bsg, bu, bsu, T.Buf(by.ptr + 2, 2 * m * f)])
+        graph = T.capture_end()
+        assert T.graph_nodes(graph)["kernel"] == launches
+        for _ in range(2):
+            T.replay(graph)
+            got = T.read(by, 0, 2 * m * f + 64).view(np.float16)
+            np.testing.assert_array_equal(got[1:1 + m * f].reshape(m, f).view(np.uint16), want.view(np.uint16))
+            assert not got[0] and not got[1 + m * f:].any()
+        for b in (*bufs, bsx, bsg, bsu, by):
+            T.free(b)
+
+
+def test_empty_sizes_launch_and_write_nothing():
+    _say("empty sizes")
+    pool = [(2, 2, 16, 32), (2, 2, 1, 32, 16), (2, 2, 16, 2), (2, 2, 16, 2)]
+    cases = [("quantize", [(0, 64), (0, 64), (0,)], 0), ("rmsnorm", [(0, 64), (64,), (0, 64), (0,)], 1),
+             ("add_rmsnorm", [(0, 64), (0, 64), (64,), (0, 64), (0,)], 1), ("linear", [(0, 64), (0,), (5, 64), (5,), (0, 5)], 0),
+             ("linear", [(5, 64), (5,), (0, 64), (0,), (5, 0)], 0), ("linear", [(0, 7), (0,), (5, 7), (5,), (0, 5)], 0),
+             ("gate_up", [(0, 64), (0,), (5, 64), (5,), (5, 64), (5,), (0, 5)], 0),
+             ("gate_up", [(3, 64), (3,), (0, 64), (0,), (0, 64), (0,), (3, 0)], 0),
+             ("kv_write", [(0, 256), (0,), (0,), (9, 32), (9, 32), *pool, (0, 2, 64), (0, 2, 64)], 0),
+             ("decode_attention", [(0, 4, 64), *pool, (0, 3), (0,), (0, 4, 64)], 1)]
+    for name, shapes, scalars in cases:
+        bufs = [T.alloc(4 * max(1, int(np.prod(s)))) for s in shapes]
+        for b in bufs:
+            T.write(b, 0, np.full(b.bytes, 0x5a, np.uint8))
+        T.launch(T.kernel("quant", name, shapes), bufs + [T.F32(1.0)] * scalars)
+        for b in bufs:
+            assert (T.read(b, 0, b.bytes) == 0x5a).all(), name
+            T.free(b)
+    # Rows of no columns have the step 0; tables of no pages, and a pool that none reads, give NaN.
+    out = run("quantize", [np.zeros((3, 0), np.float16), np.zeros((3, 0), np.int8), np.ones(3, np.float32)], outputs=[2])
+    assert not out[2].any()
+    for d in (16, 64):
+        case = _attention_case(np.random.default_rng(d), 2, 4, 2, d, 16, [20, 3])
+        case[5] = np.zeros((2, 0), np.int32)
+        assert np.isnan(_attend(*case)).all()
+
+
 @pytest.mark.parametrize("m", [3, 200])
 def test_linear_of_weights_past_4_gib(m):
     # 40000 rows of 131056: the last rows' offsets pass 32 bits. Zeros but for three rows.
