@@ -32,6 +32,7 @@ struct Q4Args {
     int CT;       // tokens per chunk (a multiple of 256)
     int pshift;   // log2(P)
     bool wide;    // one chunk a sequence, 8 wavefronts
+    int first;    // sequences are taken by length, the first of them longest first, then shortest first (0: in order)
     float c2;     // scale log2(e)
 };
 
@@ -180,10 +181,11 @@ __global__ __launch_bounds__(256) void decode_q4_any(Q4Args a) {
 // middle) and of the odd output channels at the end. step and low enter in f32: u = step (q . n) + low sum(q);
 // p step is split into two f16, so a probability keeps 22 bits.
 //
-// Bound by memory for long caches, and by VALU not far below (about 25 operations a score of 16, mostly
-// lanes of unused heads where H / G < 16).
+// Bound by memory for long caches (64 x 4096 tokens, 8 kv heads of 128: 5.6 TB/s), by latency for short ones; VALU (about 20
+// operations a token and query head, in packed lanes) is not far below.
 constexpr int TILE = 64;
 constexpr int CHUNK_MAX = 4096;  // tokens of a chunk, at most (their table entries are held in LDS)
+constexpr int RANKED = 512;      // sequences taken by length, at most
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef u32x4 u32x4u __attribute__((aligned(2)));
@@ -305,6 +307,42 @@ TSL_DEV float head_sum(float x) {
     return x + xor32(x);
 }
 
+// The sequence of slot s by length: slots 0 .. first - 1 the longest ones, longest first, the others the rest, shortest
+// first (of equal ones the first sequence is the longest). Every wavefront by itself: the r-th largest length bit by
+// bit, by counting the lengths at or above each candidate.
+TSL_DEV int by_length(const Q4Args& a, int s) {
+    constexpr int NV = RANKED / 64;
+    const int lane = threadIdx.x & 63;
+    const int r = s < a.first ? s : a.B - 1 - (s - a.first);
+    int v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        v[i] = -1;
+        if (64 * i < a.B && 64 * i + lane < a.B) v[i] = tokens_of(a, 64 * i + lane);
+    }
+    auto count = [&](int least) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+            if (64 * i < a.B) n += __popcll(__builtin_amdgcn_ballot_w64(v[i] >= least));
+        return n;
+    };
+    int at = 0;
+    for (int bit = 31 - __builtin_clz((unsigned)(a.MP * a.P)); bit >= 0; bit--)
+        if (count(at | 1 << bit) > r) at |= 1 << bit;
+    int k = r - count(at + 1), b = 0;  // the k-th of those of this length
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        if (64 * i >= a.B) break;
+        const uint64_t same = __builtin_amdgcn_ballot_w64(v[i] == at);
+        const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(v[i] == at && before == k);
+        if (hit) b = 64 * i + __builtin_ctzll(hit);
+        k -= __popcll(same);
+    }
+    return b;
+}
+
 template <int D, int QPG, int NW>
 __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q4_mfma(Q4Args a) {
     constexpr int KW = D / 32, NT = D / 16, CB = D / 8;  // words of a K row a lane; channel tiles; their bytes
@@ -322,8 +360,8 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // Chunk after chunk: workgroups go round the XCDs, and with a sequence's chunks side by side some XCDs had
     // the first ones, which all sequences have, and others the last (64 of 128-4096 tokens 57.7 us).
-    const int c = blockIdx.x / (a.B * a.G), bg = blockIdx.x % (a.B * a.G);
-    const int g = bg % a.G, b = bg / a.G;
+    const int c = blockIdx.x / (a.B * a.G), slot = blockIdx.x % (a.B * a.G);
+    const int g = slot % a.G, b = NW == 4 && a.first ? by_length(a, slot / a.G) : slot / a.G, bg = b * a.G + g;
     // The length, the chunk's table entries (t_in: where in its first page it begins) and q in
     // one round trip: none of these loads depends on another.
     const int t_lo = c * a.CT, t_in = t_lo & (a.P - 1);
@@ -594,7 +632,7 @@ __global__ __launch_bounds__(256) void decode_q4_join(Q4Args a, int qpg) {
 
 // Tokens a chunk: about two workgroups of 4 wavefronts a CU at the table's full length, which run at one time;
 // 512 at least. A workgroup costs 4 us of latencies before and after its tiles, and a second chunk the
-// join, 5 us: 64 x 128-4096 tokens, 8 kv heads of 128, chunks of 512 / 1024 / 2048 / 4096 51 / 42 / 40 / 35 us, all
+// join, 5 us (sequences in order): 64 x 128-4096 tokens, 8 kv heads of 128, chunks of 512 / 1024 / 2048 / 4096 51 / 42 / 40 / 35 us, all
 // 4096 77 / 59 / 54 / 50; one sequence of 16384 10.7 / 12.3 / 16.6 / 24.8, 16 x 100-4000 20.7 /
 // 17.4 / 17.7 / 21.7. Tables of at most ONE_CHUNK tokens are one chunk of 8 wavefronts
 // (5 x 20-333 tokens, 4 kv heads of 64, 5.4 us, 4 wavefronts 6.0).
@@ -607,6 +645,17 @@ int chunk_tokens(const TslKernel& k) {
 int nchunks(const TslKernel& k) {
     const int64_t most = k.dim("MP") * k.dim("P"), ct = chunk_tokens(k);
     return (int)std::max<int64_t>(1, (most + ct - 1) / ct);
+}
+
+// Sequences by length (by_length), where a CU has more than one workgroup, at most two, tables are long and of two chunks
+// at most: the one that comes second to a CU is short where the first is long. us, in order / by length: 64 x 128-4096
+// tokens, 8 kv heads of 128, 35.7 / 31.5, 48 of them 33.2 / 29.6, 34 26.9 / 26.7, 120 x 100-4000, 4 of 64, 32.4 / 27.8; the
+// price, one more round trip, where all have 4096 50.1 / 51.6 (by longest first for 1600 workgroups 99 / 111, for
+// tables of 16000 tokens, 4 chunks, 82.3 / 84.0: left in order).
+int ranked_first(const TslKernel& k) {
+    const int64_t B = k.dim("B"), G = k.dim("G"), cus = num_cus();
+    if (k.dim("MP") * k.dim("P") <= ONE_CHUNK || nchunks(k) > 2 || B * G <= cus || B * G > 2 * cus || B > RANKED) return 0;
+    return (int)((cus + G - 1) / G);
 }
 
 template <int D, int QPG>
@@ -665,6 +714,7 @@ int launch_decode_q4(TslKernel& k, const uint64_t* args, hipStream_t s) {
     a.B = k.dim("B"), a.H = k.dim("H"), a.G = k.dim("G"), a.NP = k.dim("NP"), a.P = k.dim("P"), a.MP = k.dim("MP");
     a.NCH = nchunks(k), a.CT = chunk_tokens(k), a.pshift = __builtin_ctz((unsigned)a.P);
     a.wide = (int64_t)a.MP * a.P <= ONE_CHUNK;
+    a.first = ranked_first(k);
     a.part = reinterpret_cast<float*>(k.scratch);
     if (a.B == 0) return 0;
     // (slices of a pool by layer or page are aligned so: 16 tokens' codes are 128 bytes at least)

@@ -483,6 +483,26 @@ def test_decode_attention(b, h, g, d, p, lens):
     _close(_attend(*case), *case)
 
 
+@pytest.mark.parametrize("b,h,g,d,p,most", [(70, 8, 4, 32, 16, 1100), (33, 8, 8, 64, 64, 3000), (130, 2, 2, 32, 16, 1040),
+                                            (300, 1, 1, 64, 16, 1025), (512, 1, 1, 32, 32, 1100), (64, 8, 8, 32, 1024, 2048),
+                                            (17, 16, 16, 32, 16, 5000)])
+def test_decode_attention_of_many_ragged_sequences(b, h, g, d, p, most):
+    # Batches of one to two workgroups a CU: ties, empty and negative lengths, lengths past the table; then all equal.
+    _say("decode_attention ragged", b, g)
+    rng = np.random.default_rng(b + g)
+    lens = rng.integers(0, 60, b)
+    lens[rng.integers(0, b, b // 3)] = 17
+    lens[[0, b // 2, b - 1]] = most, 0, most - 1
+    case = _attention_case(rng, b, h, g, d, p, lens)
+    case[6][[3, 5, 8]] = -9, 2 ** 31 - 1, -2 ** 31
+    _close(_attend(*case), *case)
+    case[6][:] = 33
+    case[5][:] = case[5][:, :1]
+    _close(_attend(*case), *case)
+    case[6][:] = 0
+    assert np.isnan(_attend(*case)).all()
+
+
 @pytest.mark.parametrize("d,h,g", [(16, 4, 2), (64, 32, 4), (128, 16, 2)])
 def test_decode_attention_odd_tables(d, h, g):
     _say("decode_attention odd tables", d)
