@@ -6,8 +6,9 @@
 //   Ks, Vs [NP, G, P, 2]:     (low, step), f16
 // With low and step factored out, a score is
 //   q . k = step (q . n) + low sum(q)
-// and an output sum(p v) = sum((p step) n) + sum(p low), so only the small whole
-// numbers n go through the products. A page outside [0, NP) reads as zeros and an
+// and an output sum(p v) = sum((p step) (n - 8)) + sum(p (low + 8 step)), so only small whole
+// numbers go through the products (values centred, for sums of codes 0 .. 15 are some 20 times the outputs that
+// they cancel to, and round accordingly). A page outside [0, NP) reads as zeros and an
 // empty sequence is 0/0 = NaN, as in decode_attention; a length past the table's
 // MP P tokens counts as MP P.
 #include "common.h"
@@ -96,8 +97,8 @@ __global__ __launch_bounds__(256) void decode_q4_any(Q4Args a) {
             const float low = h2f(a.Ks[2 * at]), step = h2f(a.Ks[2 * at + 1]);
 #pragma unroll
             for (int i = 0; i < QPG; i++) s[i] = (s[i] * step + low * qsum[i]) * a.c2;
-            vlow = h2f(a.Vs[2 * at]);
             vstep = h2f(a.Vs[2 * at + 1]);
+            vlow = __builtin_fmaf(8.0f, vstep, h2f(a.Vs[2 * at]));
         }
 #pragma unroll
         for (int i = 0; i < QPG; i++) sc[i][tid] = s[i];
@@ -137,7 +138,7 @@ __global__ __launch_bounds__(256) void decode_q4_any(Q4Args a) {
                 a.Vc + ((((long)pg * a.G + g) * (a.P / 16) + tb % a.P / 16) * D2 + j) * 16);
             for (int x = 0; x < 16; x++) {
                 const uint32_t v = (w[x >> 2] >> (8 * (x & 3))) & 255;
-                const float n0 = v & 15, n1 = v >> 4;
+                const float n0 = (int)(v & 15) - 8, n1 = (int)(v >> 4) - 8;
 #pragma unroll
                 for (int i = 0; i < QPG; i++) acc[i][0] += sc[i][16 * blk + x] * n0, acc[i][1] += sc[i][16 * blk + x] * n1;
             }
@@ -174,12 +175,13 @@ __global__ __launch_bounds__(256) void decode_q4_any(Q4Args a) {
 //   the 16 tokens of block g in order; its 16 bytes of V's layout are those tokens of a channel pair:
 //   O^T += V^T P^T, 16 channels x 16 heads a tile, channels of one parity, tokens 8 u .. 8 u + 7 of every block a step.
 //
-// A code needs no conversion: as the low bits of an f16 it is the subnormal n 2^-24, which the matrix cores
-// multiply exactly, in the next four bits n 2^-20. One shift and four ands so make 8 operand values of a word
-// (pairs of bytes 0, 2 and 1, 3, low and high nibbles): v_mfma sees n 2^-24 and 16 n 2^-24, and the
-// 16 is taken out of q's odd channels (q is scaled by a power of two into f16's
-// middle) and of the odd output channels at the end. step and low enter in f32: u = step (q . n) + low sum(q);
-// p step is split into two f16, so a probability keeps 22 bits.
+// A key's code needs no conversion: in an f16's bits 9 .. 6 it is the subnormal n 2^-18, two operations for two codes.
+// (In bits 3 .. 0, n 2^-24, one operation less for eight: but a product is aligned by its operands' exponents, a
+// subnormal's being 2^-14, and what lies 24 bits below the largest one is cut off. Sums of such codes were off by 19 times
+// 2^-23 of their largest term, one way, these by 0.2: 64 x 128-4096 tokens were 5e-5 off before the output's rounding,
+// 0.17 of the outputs another f16 than the exact one's.) A value's code goes under the exponent of 1024, from
+// where one operation takes it to n - 8. q is scaled by a power of two into f16's middle. step and low enter in f32:
+// u = step (q . n) + low sum(q); p step is split into two f16, so a probability keeps 22 bits.
 //
 // Bound by memory for long caches (64 x 4096 tokens, 8 kv heads of 128: 5.6 TB/s), by latency for short ones; VALU (about 20
 // operations a token and query head, in packed lanes) is not far below.
@@ -206,11 +208,21 @@ struct Words {  // a lane's W words of a row
     }
 };
 
-// f16 pairs of a word's codes: low nibbles of bytes (0, 2), (1, 3), then high nibbles.
+// f16 pairs of a word's codes: low nibbles of bytes (0, 2), (1, 3), then high nibbles; n 2^-18, and n - 8.
 TSL_DEV void nibbles(uint32_t w, uint32_t (&lo)[2], uint32_t (&hi)[2]) {
-    const uint32_t v = w >> 8;
-    lo[0] = w & 0x000f000fu, lo[1] = v & 0x000f000fu;
-    hi[0] = w & 0x00f000f0u, hi[1] = v & 0x00f000f0u;
+    constexpr uint32_t M = 0x03c003c0u;
+    lo[0] = (w << 6) & M, lo[1] = (w >> 2) & M;
+    hi[0] = (w << 2) & M, hi[1] = (w >> 6) & M;
+}
+// (big: 1024 twice, in a VGPR, for one v_and_or_b32 takes one scalar operand.)
+TSL_DEV void centred(uint32_t w, uint32_t big, uint32_t (&lo)[2], uint32_t (&hi)[2]) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {  // 1024 + n, 1024 + 16 n
+        const half2v l = as_half2((w >> (8 * i) & 0x000f000fu) | big), h = as_half2((w >> (8 * i) & 0x00f000f0u) | big);
+        lo[i] = __builtin_bit_cast(uint32_t, l - (half_t)1032);
+        hi[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(h, half2v{(half_t)0.0625, (half_t)0.0625},
+                                                                       half2v{(half_t)-72, (half_t)-72}));
+    }
 }
 TSL_DEV half8 half8_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return __builtin_bit_cast(half8, u32x4{a, b, c, d}); }
 
@@ -406,16 +418,16 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
     half8 qop[KW];
 #pragma unroll
     for (int w = 0; w < KW; w++) {
-        // Nibble e of a word is channel 8 w + e; its operand order: 0 4 2 6 (low) 1 5 3 7 (high, / 16).
+        // Nibble e of a word is channel 8 w + e; its operand order: 0 4 2 6 (low) 1 5 3 7 (high).
         constexpr int at[8] = {0, 4, 2, 6, 1, 5, 3, 7};
 #pragma unroll
-        for (int e = 0; e < 8; e++) qop[w][e] = (half_t)(qs[8 * w + at[e]] * (e < 4 ? up : up * 0.0625f));
+        for (int e = 0; e < 8; e++) qop[w][e] = (half_t)(qs[8 * w + at[e]] * up);
     }
     // Of the head whose scores this lane takes (l16 % TPL): u's units (a scale of 0: nearly), and low's factor.
     const int head = (lane & 48) + l16 % TPL;
-    const float unit = __builtin_ldexpf(__builtin_fabsf(a.c2), 24 - eq);
+    const float unit = __builtin_ldexpf(__builtin_fabsf(a.c2), 18 - eq);
     const float cs = __shfl(unit < 1e-37f ? 1e-37f : unit, head);  // (a NaN stays)
-    const float qz = __shfl(__builtin_ldexpf(qsum, eq - 24) * (a.c2 < 0.0f ? -1.0f : 1.0f), head);
+    const float qz = __shfl(__builtin_ldexpf(qsum, eq - 18) * (a.c2 < 0.0f ? -1.0f : 1.0f), head);
 
     const int ntiles = (len + TILE - 1) / TILE;
     const int kb = (l16 >> 2), kt = l16 & 3;  // this lane's block and token of K's tiles
@@ -443,9 +455,11 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
         for (int j = 0; j < KW; j++) x.v[j].load(vp + j * 256);
     };
 
-    float m = -INFINITY, l = 0.0f, low = 0.0f;  // maximum of u; sums of p and p low (this lane's tokens)
+    float m = -INFINITY, l = 0.0f, low = 0.0f;  // maximum of u; sums of p and p (low + 8 step) (this lane's tokens)
     float lift = 0.0f;                         // (these two of the wavefront)
     uint32_t most = 0;                         // steps below this bound need no other lift
+    uint32_t big = 0x64006400u;
+    asm("" : "+v"(big));
     float4v acc[NT];
 #pragma unroll
     for (int i = 0; i < NT; i++) acc[i] = float4v{};
@@ -517,7 +531,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(u[4 * t + r], cs, off));
                 const uint32_t pair = x.vs.get(4 * t + r);
                 l += p;
-                low = __builtin_fmaf(p, lo_h(pair), low);
+                low = __builtin_fmaf(p, __builtin_fmaf(8.0f, hi_h(pair), lo_h(pair)), low);
                 const float w = p * hi_h(pair);
                 h[r] = (half_t)w;
                 e[r] = (half_t)(w - (float)h[r]);
@@ -538,8 +552,8 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
 #pragma unroll
             for (int j = 0; j < D / 32; j++) {
                 uint32_t l0[2], h0[2], l1[2], h1[2];
-                nibbles(x.v[j].w[2 * s], l0, h0);
-                nibbles(x.v[j].w[2 * s + 1], l1, h1);
+                centred(x.v[j].w[2 * s], big, l0, h0);
+                centred(x.v[j].w[2 * s + 1], big, l1, h1);
                 const half8 even = half8_of(l0[0], l0[1], l1[0], l1[1]), odd = half8_of(h0[0], h0[1], h1[0], h1[1]);
                 acc[2 * j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, hp, acc[2 * j], 0, 0, 0);
                 acc[2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, hp, acc[2 * j + 1], 0, 0, 0);
@@ -567,8 +581,7 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
             for (int e = 0; e < 2; e++)
 #pragma unroll
                 for (int r = 0; r < 4; r++)
-                    red[wave][l16][2 * (16 * j + 4 * g4 + r) + e] =
-                        __builtin_fmaf(acc[2 * j + e][r], e ? 0x1p20f : 0x1p24f, low);
+                    red[wave][l16][2 * (16 * j + 4 * g4 + r) + e] = acc[2 * j + e][r] + low;
         if (g4 == 0) red[wave][l16][D] = m * cs - lift, red[wave][l16][D + 1] = l;
     }
     __syncthreads();

@@ -101,3 +101,56 @@ def attention(q, kn, vn, ks, vs, table, lens, scale):
             kl = np.where(ok[:, None], np.abs(k) + 2 * np.abs(ks[pg, gg, t % p, :1].astype(np.float64)), 0.0)
             top[i, hh] = (kl @ np.abs(q[i, hh].astype(np.float64))).max() * abs(float(scale))
     return out, mag, top
+
+
+def attention_error(q, kn, vn, ks, vs, table, lens, scale):
+    """softmax(scale q K^T) V in f64 (NaN rows for empty sequences), and the root mean square of what f32 arithmetic is off
+    by before the output's rounding to f16, element by element.
+
+    Token t's score step (q . n) + low sum(q) is off by one rounding of each term and of the sum, and by those of q . n's
+    partial sums (a term's size, |q| 15 step at most): its probability by r_t = 2^-24 (4 + scale (|step q . n| +
+    |low sum(q)| + |score| + 15 step max|q|)) of itself, each token's for itself, which moves an output by
+    p_t r_t |v_t - out|. The sums over tokens are of centred values, sum p step (n - 8) and sum p (low + 8 step): a chain of N roundings
+    of a sum that grows adds to sqrt(N / 3) half-steps, 4 of the sum of magnitudes for N = 48."""
+    b, h, d = q.shape
+    npg, g, p, _ = kn.shape
+    out, rms = np.full((b, h, d), np.nan), np.zeros((b, h, d))
+    for i in range(b):
+        n = min(max(int(lens[i]), 0), table.shape[1] * p)
+        if n == 0:
+            continue
+        t = np.arange(n)
+        page = table[i, t // p]
+        ok = ((page >= 0) & (page < npg))[:, None]
+        pg = np.where(ok[:, 0], page, 0)
+        for gg in range(g):
+            (kc, kp), (vc, vp) = ((c[pg, gg, t % p].astype(np.float64), np.where(ok, x[pg, gg, t % p].astype(np.float64), 0.0))
+                                  for c, x in ((kn, ks), (vn, vs)))
+            v, mag = vp[:, :1] + vp[:, 1:] * vc, np.abs(vp[:, 1:] * (vc - 8)) + np.abs(vp[:, :1] + 8 * vp[:, 1:])
+            for hh in range(gg * (h // g), (gg + 1) * (h // g)):
+                qq = q[i, hh].astype(np.float64)
+                a, c = kp[:, 1] * (kc @ qq), kp[:, 0] * qq.sum()
+                e = np.exp((a + c) * float(scale) - ((a + c) * float(scale)).max())
+                e /= e.sum()
+                r = 4 + abs(float(scale)) * (np.abs(a) + np.abs(c) + np.abs(a + c) + 15 * kp[:, 1] * np.abs(qq).max())
+                out[i, hh] = e @ v
+                rms[i, hh] = 2.0 ** -24 * np.sqrt(((e * r) ** 2) @ (v - out[i, hh]) ** 2 + (4 * (e @ mag)) ** 2)
+    return out, rms
+
+
+def f16_steps(x):
+    """The distance of f16's neighbours at x (f64)."""
+    return 2.0 ** (np.where(x == 0, -13, np.maximum(np.frexp(np.abs(x))[1], -13)) - 11.0)
+
+
+def within_f32(got, want, rms):
+    """Whether f16 outputs are the exact ones as f32 arithmetic leaves them (attention_error): none further off than
+    half a step of f16 and 8 times `rms`; and how many of them are another f16 than the exact one's, and how many may be: an
+    error moves an output over a border between two f16 with the odds error / step, its mean magnitude is `rms` at
+    most, and their number varies by its square root."""
+    live = ~np.isnan(want)
+    near = np.abs(got - want) <= f16_steps(want) / 2 + 8 * rms
+    moved = (got != want.astype(np.float16)) & live
+    odds = np.where(live, np.minimum(1.0, rms / f16_steps(want)), 0.0)
+    most = odds.sum() + 4 * np.sqrt(odds.sum()) + 1
+    return bool((np.isnan(got) == np.isnan(want)).all() and (near | ~live).all()), int(moved.sum()), float(most)
