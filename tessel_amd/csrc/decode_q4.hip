@@ -532,7 +532,8 @@ __global__ __launch_bounds__(64 * NW, D == 128 || NW == 8 ? 2 : 3) void decode_q
                 const uint32_t pair = x.vs.get(4 * t + r);
                 l += p;
                 low = __builtin_fmaf(p, __builtin_fmaf(8.0f, hi_h(pair), lo_h(pair)), low);
-                const float w = p * hi_h(pair);
+                float w = p * hi_h(pair);
+                asm("" : "+v"(w));  // (both halves of one f32 value: else one comes of the product rounded to f16 at once)
                 h[r] = (half_t)w;
                 e[r] = (half_t)(w - (float)h[r]);
             }
