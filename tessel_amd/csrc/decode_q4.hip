@@ -709,7 +709,7 @@ int setup_decode_q4(TslKernel& k) {
         return tsl_fail(-2, "quant/decode_attention: H / G must be 1, 2, 4, 8 or 16");
     if (k.dim("NP") == 0) return tsl_fail(-2, "quant/decode_attention: a pool of no pages");
     // (a launch holds less than 2^32 work-items, 512 at most for each of these)
-    if (MP > INT_MAX / k.dim("P") || B * H > (1 << 22) || B * G * nchunks(k) > (1 << 22))
+    if (MP > INT_MAX / k.dim("P") || B > (1 << 22) || H > (1 << 22) || B * H > (1 << 22) || B * G * nchunks(k) > (1 << 22))
         return tsl_fail(-2, "quant/decode_attention: at most 2^31 - 1 tokens a table and 2^22 (sequence, head, chunk)s");
     return nchunks(k) > 1 ? tsl_scratch(k, (size_t)B * H * nchunks(k) * (2 + k.dim("D")) * sizeof(float)) : 0;
 }

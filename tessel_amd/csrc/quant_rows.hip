@@ -474,6 +474,7 @@ int check_cache_q4(const TslKernel& k) {
         return tsl_fail(-2, "quant/" + k.name + ": head dimension " + std::to_string(D) + " unsupported (16, 32, 64 or 128)");
     if (k.dim("D2") * 2 != D) return tsl_fail(-2, "quant/" + k.name + ": D2 must be D / 2");
     if (P % 16 != 0) return tsl_fail(-2, "quant/" + k.name + ": pages must hold a multiple of 16 tokens");
+    if (P > (1 << 30)) return tsl_fail(-2, "quant/" + k.name + ": pages hold at most 2^30 tokens");
     if (k.dim("PB") * 16 != P) return tsl_fail(-2, "quant/" + k.name + ": PB must be P / 16");
     if (k.dim("G") <= 0 || k.dim("NP") > INT_MAX || k.dim("G") > INT_MAX)
         return tsl_fail(-2, "quant/" + k.name + ": G and NP must be positive and below 2^31");
