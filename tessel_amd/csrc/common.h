@@ -148,7 +148,7 @@ struct TslKernel {
 typedef int (*tsl_launcher)(TslKernel& k, const uint64_t* args, hipStream_t s);
 typedef int (*tsl_preparer)(TslKernel& k);  // optional: scratch sizing at tsl_kernel time
 
-// Gives handle k a device buffer of its own (opening the device; 0 bytes: neither).
+// Gives handle k a device buffer for the time of a launch, which it shares with others (opening the device; 0 bytes: neither).
 int tsl_scratch(TslKernel& k, size_t bytes);
 
 // Compute units of the current device (runtime.hip; cached).

@@ -9,6 +9,7 @@
 //
 // An MFMA operand is 16 bytes a lane here as in the f16 products: lane l holds
 // row l % 16 and k 16 (l / 16) .. +15 of a 64-k substep.
+#include "../../include/tessel.h"
 #include "common.h"
 
 #include <algorithm>
@@ -823,7 +824,7 @@ template <int EPI>
 int run_gemm8(Gemm8 a, TslKernel& k, hipStream_t s) {
     if (a.M == 0 || a.N == 0) return 0;
     if (k.scratch) {
-        const int kp = (a.K + 127) / 128 * 128, rows = (int)(k.scratch_bytes / kp);
+        const int kp = (a.K + 127) / 128 * 128, rows = a.M + (EPI == Q_SWIGLU ? 2 : 1) * a.N;
         int8_t* out = reinterpret_cast<int8_t*>(k.scratch);
         hipLaunchKernelGGL(pack_rows_kernel, dim3((unsigned)std::min((rows + 3) / 4, 1 << 16)), dim3(256), 0, s, a, out, kp, rows);
         if (int r = TSL_LAUNCHED("quant product rows")) return r;
@@ -847,7 +848,11 @@ int setup_i8(TslKernel& k, const char* n) {
     if ((k.dim("M") + 63) * (k.dim(n) + 31) >= (1LL << 34)) return tsl_fail(-2, "quant/" + k.name + ": at most 2^34 outputs");
     Gemm8 a{};
     a.M = (int)k.dim("M"), a.N = (int)k.dim(n), a.K = (int)k.dim("K");
-    return tsl_scratch(k, packed_bytes<EPI>(a));
+    const size_t bytes = packed_bytes<EPI>(a);
+    if (!bytes) return 0;
+    if (int r = tsl_open()) return r;
+    (void)tsl_scratch(k, bytes);  // (no memory for a copy: gemm_i8_any, which needs none)
+    return 0;
 }
 
 }  // namespace

@@ -13,6 +13,7 @@
 // they change results (softmax/rmsnorm BC, the columns a row kernel reads).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdio>
 #include <cstring>
 #include <map>
@@ -71,11 +72,29 @@ int setup_linear_q8(TslKernel&);
 int setup_gate_up_q8(TslKernel&);
 int setup_decode_q4(TslKernel&);
 
+// One buffer serves all handles: launches follow one another on one stream, and none leaves anything there for a later one.
+// (A buffer a handle held as many copies of a weight matrix as there were row counts.) A handle keeps the buffer that it was made
+// with, whose address captured graphs have, so a buffer that has become too small stays; each is half as large
+// again as the one before at least, so that all of them are at most three times the largest.
 int tsl_scratch(TslKernel& k, size_t bytes) {
+    static void* held = nullptr;
+    static size_t size = 0;
     if (!bytes) return 0;
     if (int r = tsl_open()) return r;
-    if (int r = tsl_hip_check(hipMalloc(&k.scratch, bytes), (k.file + "/" + k.name + " scratch").c_str())) return r;
-    k.scratch_bytes = bytes;
+    if (size < bytes) {
+        void* p = nullptr;
+        size_t n = std::max(bytes, size + size / 2);
+        if (n > bytes && hipMalloc(&p, n) != hipSuccess) {
+            (void)hipGetLastError();
+            p = nullptr;
+        }
+        if (!p) {
+            n = bytes;
+            if (int r = tsl_hip_check(hipMalloc(&p, n), (k.file + "/" + k.name + " scratch").c_str())) return r;
+        }
+        held = p, size = n;
+    }
+    k.scratch = held, k.scratch_bytes = bytes;
     return 0;
 }
 
