@@ -287,7 +287,14 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rmsnorm_q8_kernel(const u
 //
 // A workgroup a token, D / 4 lanes a head: lane j holds channels 2j, 2j + 1 and their rotary
 // partners D/2 on, which are the bytes j and D/4 + j of the cache's row. Bound by its chain of loads
-// (position, slot, rows, tables).
+// (position, slot, rows, tables) for few tokens.
+//
+// Of rows that name one slot the last is kept. Up to LOOK tokens every workgroup looks through the later rows' slots (T^2 / 2
+// loads, one launch); beyond, a table of each slot's last row is made first (a hash table of 2 T to 4 T entries, two launches
+// more). us, look / table: 4 kv heads of 64, 4096 tokens 9.2 / 12.0, 6000 12.4 / 13.4, 8192 17.2 / 15.5, 16384 41 / 22.9; 8 of 128,
+// 4096 23.5 / 23.2, 8192 44.5 / 37, 16384 97 / 65.
+constexpr int LOOK = 6144;
+
 struct KvArgs {
     const u16* QKV;
     const int *pos, *slot;
@@ -296,7 +303,48 @@ struct KvArgs {
     u16 *Ks, *Vs, *K, *V;
     int T, W, NPOS, G, P;
     long NS;
+    unsigned long long* last;  // [1 << bits] (slot + 1) << 32 | its last row, 0: empty (null: no table)
+    int bits;
 };
+
+// A slot's first place in the table, of 2^bits (Fibonacci hashing: neighbouring slots lie far apart).
+TSL_DEV uint32_t place_of(int slot, int bits) { return ((uint32_t)slot * 2654435769u) >> (32 - bits); }
+
+__global__ __launch_bounds__(256) void kv_clear_kernel(KvArgs a) {
+    u32x4* to = reinterpret_cast<u32x4*>(a.last);
+    const long n = 1L << (a.bits - 1);
+    for (long i = blockIdx.x * 256L + threadIdx.x; i < n; i += gridDim.x * 256L) to[i] = u32x4{0, 0, 0, 0};
+}
+
+// Every row's slot into the table, with the largest row number of each: whatever order they come in, the table holds the
+// same for each slot. At most T of its 2 T places or more are taken, so that a free one is always met.
+__global__ __launch_bounds__(256) void kv_last_kernel(KvArgs a) {
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= a.T) return;
+    const int at = a.slot[t];
+    if (at < 0 || at >= a.NS) return;
+    const unsigned long long mine = (unsigned long long)(uint32_t)(at + 1u) << 32 | (uint32_t)t;
+    const uint32_t mask = (1u << a.bits) - 1;
+    for (uint32_t i = place_of(at, a.bits), n = 0; n <= mask; i = (i + 1) & mask, n++) {
+        const unsigned long long was = atomicCAS(a.last + i, 0ull, mine);
+        if (was == 0) return;
+        if (was >> 32 == mine >> 32) {
+            atomicMax(a.last + i, mine);
+            return;
+        }
+    }
+}
+
+// The last row that names slot `at` (which one does).
+TSL_DEV int last_of(const KvArgs& a, int at) {
+    const uint32_t mask = (1u << a.bits) - 1, key = at + 1u;
+    for (uint32_t i = place_of(at, a.bits), n = 0; n <= mask; i = (i + 1) & mask, n++) {
+        const unsigned long long e = a.last[i];
+        if ((uint32_t)(e >> 32) == key) return (int)(uint32_t)e;
+        if (e == 0) break;
+    }
+    return -1;
+}
 
 TSL_DEV u16 rotate(float a, float c, float b, float s) {  // a c + b s
     float y = __builtin_fmaf(a, c, b * s);
@@ -304,23 +352,28 @@ TSL_DEV u16 rotate(float a, float c, float b, float s) {  // a c + b s
     return f2h(y);
 }
 
-template <int D>
+// TABLE: a.last is made.
+template <int D, bool TABLE>
 __global__ __launch_bounds__(512) void kv_write_q4_kernel(KvArgs a) {
     constexpr int D2 = D / 2, LPH = D / 4;
     typedef float float2u __attribute__((ext_vector_type(2), aligned(4)));
     const int t = blockIdx.x, nt = blockDim.x;
     const int p = a.pos[t], at = a.slot[t];
-    // Rows that name one slot: the last is kept. Every thread looks at its share of the later rows, 8
-    // loads at a time (2003 tokens 8.7 us with one).
-    bool later = false;
-    for (int u = t + 1 + threadIdx.x; u < a.T; u += 8 * nt) {
-        int other[8];
+    bool keep;
+    if constexpr (TABLE) {
+        keep = at >= 0 && at < a.NS && last_of(a, at) == t;
+    } else {
+        // Every thread looks at its share of the later rows, 8 loads at a time (2003 tokens 8.7 us with one).
+        bool later = false;
+        for (int u = t + 1 + threadIdx.x; u < a.T; u += 8 * nt) {
+            int other[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) other[i] = u + i * nt < a.T ? a.slot[u + i * nt] : -1;
+            for (int i = 0; i < 8; i++) other[i] = u + i * nt < a.T ? a.slot[u + i * nt] : -1;
 #pragma unroll
-        for (int i = 0; i < 8; i++) later = later || other[i] == at;
+            for (int i = 0; i < 8; i++) later = later || other[i] == at;
+        }
+        keep = !__syncthreads_or(later) && at >= 0 && at < a.NS;
     }
-    const bool keep = !__syncthreads_or(later) && at >= 0 && at < a.NS;
     const int lane = threadIdx.x % LPH;
     const long page = keep ? at / a.P : 0;
     const int off = keep ? at % a.P : 0;
@@ -442,6 +495,24 @@ int run_rmsnorm_q8(TslKernel& k, const u16* X, const uint64_t* a, hipStream_t s)
     return TSL_LAUNCHED("quant rmsnorm");
 }
 
+template <bool TABLE>
+int run_kv_write(const KvArgs& r, int64_t D, hipStream_t s) {
+    const int lanes = (int)std::min<long>(512, (2L * r.G * (D / 4) + 63) / 64 * 64);
+    switch (D) {
+        case 16: hipLaunchKernelGGL((kv_write_q4_kernel<16, TABLE>), dim3(r.T), dim3(lanes), 0, s, r); break;
+        case 32: hipLaunchKernelGGL((kv_write_q4_kernel<32, TABLE>), dim3(r.T), dim3(lanes), 0, s, r); break;
+        case 64: hipLaunchKernelGGL((kv_write_q4_kernel<64, TABLE>), dim3(r.T), dim3(lanes), 0, s, r); break;
+        default: hipLaunchKernelGGL((kv_write_q4_kernel<128, TABLE>), dim3(r.T), dim3(lanes), 0, s, r); break;
+    }
+    return TSL_LAUNCHED("quant kv_write");
+}
+
+int table_bits(int T) {  // 2 T to 4 T places
+    int bits = 1;
+    while ((1L << bits) < 2L * T) bits++;
+    return bits;
+}
+
 }  // namespace
 
 int setup_quantize(TslKernel& k) { return check_rows(k, "M", "K"); }
@@ -487,7 +558,7 @@ int setup_kv_write_q4(TslKernel& k) {
         return tsl_fail(-2, "quant/kv_write: rows of W = " + std::to_string(k.dim("W")) + " hold no 2 G D keys and values");
     if (k.dim("T") >= (1 << 23) || k.dim("W") > INT_MAX || k.dim("NPOS") > INT_MAX)
         return tsl_fail(-2, "quant/kv_write: tokens below 2^23 and sizes below 2^31");
-    return 0;
+    return k.dim("T") > LOOK ? tsl_scratch(k, sizeof(unsigned long long) << table_bits((int)k.dim("T"))) : 0;
 }
 
 int launch_kv_write_q4(TslKernel& k, const uint64_t* a, hipStream_t s) {
@@ -498,13 +569,13 @@ int launch_kv_write_q4(TslKernel& k, const uint64_t* a, hipStream_t s) {
     r.Kc = P<uint8_t>(a[5]), r.Vc = P<uint8_t>(a[6]), r.Ks = P<u16>(a[7]), r.Vs = P<u16>(a[8]);
     r.K = P<u16>(a[9]), r.V = P<u16>(a[10]);
     if (r.T == 0) return 0;
-    const int D = k.dim("D");
-    const int lanes = (int)std::min<long>(512, (2L * r.G * (D / 4) + 63) / 64 * 64);
-    switch (D) {
-        case 16: hipLaunchKernelGGL(kv_write_q4_kernel<16>, dim3(r.T), dim3(lanes), 0, s, r); break;
-        case 32: hipLaunchKernelGGL(kv_write_q4_kernel<32>, dim3(r.T), dim3(lanes), 0, s, r); break;
-        case 64: hipLaunchKernelGGL(kv_write_q4_kernel<64>, dim3(r.T), dim3(lanes), 0, s, r); break;
-        default: hipLaunchKernelGGL(kv_write_q4_kernel<128>, dim3(r.T), dim3(lanes), 0, s, r); break;
+    if (r.T > LOOK) {
+        r.last = static_cast<unsigned long long*>(k.scratch), r.bits = table_bits(r.T);
+        const unsigned clear = (unsigned)std::min<long>(1024, ((1L << (r.bits - 1)) + 255) / 256);
+        hipLaunchKernelGGL(kv_clear_kernel, dim3(clear), dim3(256), 0, s, r);
+        if (int e = TSL_LAUNCHED("quant kv_write table")) return e;
+        hipLaunchKernelGGL(kv_last_kernel, dim3((unsigned)((r.T + 255) / 256)), dim3(256), 0, s, r);
+        if (int e = TSL_LAUNCHED("quant kv_write table")) return e;
     }
-    return TSL_LAUNCHED("quant kv_write");
+    return r.last ? run_kv_write<true>(r, k.dim("D"), s) : run_kv_write<false>(r, k.dim("D"), s);
 }
