@@ -75,6 +75,12 @@ int tsl_kernel(const char* file, const char* name, int nshapes, const int* ranks
                int* handle);
 /* The cache key of a handle, into buf. */
 int tsl_kernel_key(int handle, char* buf, size_t len);
+/* The form that a launch of a quant/linear or quant/gate_up handle takes, by
+ * its sizes and whether its operands begin at multiples of 16 bytes, into
+ * buf: a tile ("64x64" to "256x256"), "skinny" and its rows, "any" and its
+ * groups along K, "copied" before a form whose rows are copied first. All
+ * forms give the same bits; tests say by it which of them they ran. */
+int tsl_product_form(int handle, int aligned, char* buf, size_t len);
 /*
  * Launches kernel `handle` asynchronously on the library stream with one
  * 64-bit argument per .tl parameter, in declaration order: arrays are

@@ -52,7 +52,7 @@ EXPORTS = [
     "tsl_checkpoint_save", "tsl_json_roundtrip", "tsl_rng_new", "tsl_rng_bits", "tsl_rng_tensor",
     "tsl_time_each", "tsl_engine_profile", "tsl_engine_profile_rows", "tsl_schedule_trace",
     "tsl_graph_nodes", "tsl_engine_graphs", "tsl_engine_fallbacks", "tsl_engine_step_times", "tsl_probe_mfma", "tsl_probe_mfma16", "tsl_probe_stream",
-    "tsl_decode_attention_noalloc",
+    "tsl_decode_attention_noalloc", "tsl_product_form",
 ]
 
 
@@ -104,6 +104,7 @@ def _declare(L):
     L.tsl_kernel.argtypes = [ctypes.c_char_p, ctypes.c_char_p, _INT, ctypes.POINTER(_INT), ctypes.POINTER(_I64), _INT,
                              ctypes.POINTER(ctypes.c_char_p), ctypes.POINTER(_I64), _INT, ctypes.POINTER(_INT)]
     L.tsl_kernel_key.argtypes = [_INT, ctypes.c_char_p, ctypes.c_size_t]
+    L.tsl_product_form.argtypes = [_INT, _INT, ctypes.c_char_p, ctypes.c_size_t]
     L.tsl_launch.argtypes = [_INT, ctypes.POINTER(_U64), _INT]
     L.tsl_time_launches.argtypes = [_INT, ctypes.POINTER(_U64), _INT, _INT, ctypes.POINTER(ctypes.c_float)]
     L.tsl_capture_end.argtypes = [ctypes.POINTER(_INT)]
@@ -228,6 +229,14 @@ def kernel(file, name, shapes, meta=(), warps=4):
     check(lib().tsl_kernel(file.encode(), name.encode(), len(shapes), ranks, dims, len(meta), names, vals, int(warps),
                            ctypes.byref(h)))
     return Kernel(h.value, name)
+
+
+def product_form(k, aligned=True):
+    """The form that a launch of a quant/linear or quant/gate_up kernel takes
+    (tsl_product_form), its operands at multiples of 16 bytes or not."""
+    buf = ctypes.create_string_buffer(64)
+    check(lib().tsl_product_form(k.handle, int(aligned), buf, 64))
+    return buf.value.decode()
 
 
 def launch(k, args):

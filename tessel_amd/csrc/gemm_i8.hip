@@ -857,6 +857,23 @@ int setup_i8(TslKernel& k, const char* n) {
 
 }  // namespace
 
+// What run_gemm8 launches, as tsl_product_form names it.
+template <int EPI>
+static std::string form_of(const TslKernel& k, const char* n, bool aligned) {
+    static const char* const names[] = {"64x64", "64x128", "128x128", "256x128", "256x256"};
+    Gemm8 a{};
+    a.M = (int)k.dim("M"), a.N = (int)k.dim(n), a.K = (int)k.dim("K");
+    if (a.M == 0 || a.N == 0) return "none";
+    const bool copied = k.scratch != nullptr;
+    if (copied) a.K = (a.K + 127) / 128 * 128;
+    else if (!aligned || a.K % 16 || a.K == 0) return any_tiles<EPI>(a) <= num_cus() ? "any 4" : "any 2";
+    const int form = plan_aligned<EPI>(a).form;
+    return (copied ? "copied " : "") + (form < 5 ? std::string(names[form]) : "skinny " + std::to_string((a.M + 15) / 16 * 16));
+}
+std::string quant_product_form(const TslKernel& k, bool aligned) {
+    return k.name == "linear" ? form_of<Q_LINEAR>(k, "N", aligned) : form_of<Q_SWIGLU>(k, "F", aligned);
+}
+
 int setup_linear_q8(TslKernel& k) { return setup_i8<Q_LINEAR>(k, "N"); }
 int setup_gate_up_q8(TslKernel& k) { return setup_i8<Q_SWIGLU>(k, "F"); }
 

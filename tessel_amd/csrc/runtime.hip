@@ -71,6 +71,7 @@ int setup_kv_write_q4(TslKernel&);
 int setup_linear_q8(TslKernel&);
 int setup_gate_up_q8(TslKernel&);
 int setup_decode_q4(TslKernel&);
+std::string quant_product_form(const TslKernel&, bool aligned);
 
 // One buffer serves all handles: launches follow one another on one stream, and none leaves anything there for a later one.
 // (A buffer a handle held as many copies of a weight matrix as there were row counts.) A handle keeps the buffer that it was made
@@ -573,6 +574,15 @@ int tsl_kernel(const char* file, const char* name, int nshapes, const int* ranks
 int tsl_kernel_key(int handle, char* buf, size_t len) {
     if (handle < 0 || handle >= (int)g.kernels.size()) return tsl_fail(TSL_ERR_ARG, "no such kernel handle");
     snprintf(buf, len, "%s", g.kernels[handle]->key.c_str());
+    return 0;
+}
+
+int tsl_product_form(int handle, int aligned, char* buf, size_t len) {
+    if (handle < 0 || handle >= (int)g.kernels.size()) return tsl_fail(TSL_ERR_ARG, "no such kernel handle");
+    const TslKernel& k = *g.kernels[handle];
+    if (k.file != "quant" || (k.name != "linear" && k.name != "gate_up"))
+        return tsl_fail(TSL_ERR_ARG, k.file + "/" + k.name + " is no product of 8-bit rows");
+    snprintf(buf, len, "%s", quant_product_form(k, aligned != 0).c_str());
     return 0;
 }
 
