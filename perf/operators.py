@@ -212,11 +212,14 @@ CALLS = {"linear": ("linear", ("x", "sx", "w", "sw", "y"), ()),
 
 def _call(state):
     """The kernel's handle and arguments, which a program keeps with its buffers. torch's own work goes to the
-    library's stream from here on, so what reads a kernel's outputs follows it."""
+    library's stream from here on, so what reads a kernel's outputs follows it; what made the inputs on another
+    stream is waited for, there."""
     import tessel_amd as T
 
     T.open()
-    torch.cuda.set_stream(torch.cuda.ExternalStream(T.lib().tsl_stream()))
+    stream = torch.cuda.ExternalStream(T.lib().tsl_stream())
+    stream.wait_stream(torch.cuda.current_stream())
+    torch.cuda.set_stream(stream)
     name, arrays, scalars = CALLS["add_norm" if "x" in state and state["kind"] == "norm" else state["kind"]]
     kernel = T.kernel("quant", name, [tuple(state[a].shape) for a in arrays])
     args = [T.Buf(state[a].data_ptr(), state[a].numel() * state[a].element_size()) for a in arrays]
