@@ -594,6 +594,7 @@ int tsl_launch(int handle, const uint64_t* args, int nargs) {
         o << k.name << ": " << nargs << " arguments for " << k.nparams << " parameters";
         return tsl_fail(TSL_ERR_ARG, o.str());
     }
+    if (!g.open) NEED_OPEN();  // (handles without scratch are made before the device is opened)
     return g.launchers[handle](k, args, g.stream);
 }
 

@@ -28,3 +28,18 @@ def test_refusals(name, shapes, msg):
 def test_the_largest_pages_are_taken():
     T.kernel("quant", "kv_write", _write(p=2 ** 30))
     T.kernel("quant", "decode_attention", _decode(b=0, p=2 ** 30, mp=1))
+
+
+def test_a_launch_opens_the_device():
+    # (A handle that needs no scratch is made without one; a launch before anything else went to the null stream of whatever
+    # device was current, which tsl_sync does not wait for. Rows of none: nothing is launched.)
+    k = T.kernel("quant", "quantize", [[0, 64], [0, 64], [0]])
+
+    def says(f):
+        try:
+            return f()
+        except T.TesselError as e:
+            return str(e)
+
+    launched = says(lambda: T.launch(k, [T.Buf(0, 0)] * 3))
+    assert launched == says(T.open)
