@@ -181,10 +181,11 @@ __global__ __launch_bounds__(256) void decode_q4_any(Q4Args a) {
 // 2^-23 of their largest term, one way, these by 0.2: 64 x 128-4096 tokens were 5e-5 off before the output's rounding,
 // 0.17 of the outputs another f16 than the exact one's.) A value's code goes under the exponent of 1024, from
 // where one operation takes it to n - 8. q is scaled by a power of two into f16's middle. step and low enter in f32:
-// u = step (q . n) + low sum(q); p step is split into two f16, so a probability keeps 22 bits.
+// u = step (q . n) + low sum(q); p step is split into two f16, so a probability keeps 22 bits (beside a step up to 2^16 times
+// its token's; a further one leaves it those above 2^-38 of that step).
 //
-// Bound by memory for long caches (64 x 4096 tokens, 8 kv heads of 128: 5.6 TB/s), by latency for short ones; VALU (about 20
-// operations a token and query head, in packed lanes) is not far below.
+// Bound by memory for long caches (64 x 4096 tokens, 8 kv heads of 128: 5.4 TB/s), by latency for short ones; VALU (about 20
+// operations a token and query head, in packed lanes, and 17 for 8 codes of keys and 8 of values) is not far below.
 constexpr int TILE = 64;
 constexpr int CHUNK_MAX = 4096;  // tokens of a chunk, at most (their table entries are held in LDS)
 constexpr int RANKED = 512;      // sequences taken by length, at most
@@ -646,10 +647,10 @@ __global__ __launch_bounds__(256) void decode_q4_join(Q4Args a, int qpg) {
 
 // Tokens a chunk: about two workgroups of 4 wavefronts a CU at the table's full length, which run at one time;
 // 512 at least. A workgroup costs 4 us of latencies before and after its tiles, and a second chunk the
-// join, 5 us (sequences in order): 64 x 128-4096 tokens, 8 kv heads of 128, chunks of 512 / 1024 / 2048 / 4096 51 / 42 / 40 / 35 us, all
-// 4096 77 / 59 / 54 / 50; one sequence of 16384 10.7 / 12.3 / 16.6 / 24.8, 16 x 100-4000 20.7 /
-// 17.4 / 17.7 / 21.7. Tables of at most ONE_CHUNK tokens are one chunk of 8 wavefronts
-// (5 x 20-333 tokens, 4 kv heads of 64, 5.4 us, 4 wavefronts 6.0).
+// join, 5 us (sequences in order): 64 x 128-4096 tokens, 8 kv heads of 128, chunks of 512 / 1024 / 2048 / 4096 55 / 45 / 45 / 39 us, all
+// 4096 82 / 63 / 57 / 52; one sequence of 16384 11.3 / 13.2 / 18.4 / 28.1, 16 x 100-4000 22.2 /
+// 18.8 / 19.4 / 24.9. Tables of at most ONE_CHUNK tokens are one chunk of 8 wavefronts
+// (5 x 20-333 tokens, 4 kv heads of 64, 5.8 us, 4 wavefronts 6.5).
 constexpr int ONE_CHUNK = 1024;
 int chunk_tokens(const TslKernel& k) {
     const int64_t bg = std::max<int64_t>(1, k.dim("B") * k.dim("G")), most = k.dim("MP") * k.dim("P");
@@ -663,9 +664,9 @@ int nchunks(const TslKernel& k) {
 
 // Sequences by length (by_length), where a CU has more than one workgroup, at most two, tables are long and of two chunks
 // at most: the one that comes second to a CU is short where the first is long. us, in order / by length: 64 x 128-4096
-// tokens, 8 kv heads of 128, 35.7 / 31.5, 48 of them 33.2 / 29.6, 34 26.9 / 26.7, 120 x 100-4000, 4 of 64, 32.4 / 27.8; the
-// price, one more round trip, where all have 4096 50.1 / 51.6 (by longest first for 1600 workgroups 99 / 111, for
-// tables of 16000 tokens, 4 chunks, 82.3 / 84.0: left in order).
+// tokens, 8 kv heads of 128, 39.5 / 32.9, 48 of them 37.0 / 32.3, 34 30.2 / 29.3, 120 x 100-4000, 4 of 64, 35.9 / 30.3; the
+// price, one more round trip, where all have 4096 52.0 / 52.9 (by longest first for 1600 workgroups 12 % more, for
+// tables of 16000 tokens, 4 chunks, 2 %: left in order).
 int ranked_first(const TslKernel& k) {
     const int64_t B = k.dim("B"), G = k.dim("G"), cus = num_cus();
     if (k.dim("MP") * k.dim("P") <= ONE_CHUNK || nchunks(k) > 2 || B * G <= cus || B * G > 2 * cus || B > RANKED) return 0;

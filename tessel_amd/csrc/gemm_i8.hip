@@ -707,9 +707,8 @@ int run_tile(const Gemm8& a, hipStream_t s) {
     return TSL_LAUNCHED("quant product");
 }
 
-// The time of a product by each form, in us, from its LDS traffic, which bounds
-// them all (128 bytes a clock and CU; a larger tile reads each staged row more often):
-// a step of 128 k costs what it measured on one busy CU, 0.4 of it more with all CUs busy
+// The time of a product by each form, in us, from its steps (no form fills the matrix cores or LDS; each is bound by its
+// chain of loads, LDS reads and barriers): a step of 128 k costs what it measured on one busy CU, 0.4 of it more with all CUs busy
 // (the clock falls), and a product takes as many rounds of them as its tiles need on the CUs:
 //   64 x 64 .18 us, 64 x 128 .26, 128 x 128 .37, 256 x 128 .60, 256 x 256 .91, and 3 to 6 us for
 // filling, the epilogue and the launch. The skinny form stages 16 rows of W and all of X a block, 54 KB
