@@ -113,3 +113,18 @@ def test_every_edge_of_a_batch_by_length():
         case[1][page, :, t % p] = np.where(case[0][i] > 0, 15, 0)  # (a query head a kv head)
         case[3][page, :, t % p] = np.array([-7.5, 1.0]) * 0.7
     assert _moved(case)[0]
+
+
+@pytest.mark.parametrize("b,h,g,d,most", [(64, 32, 8, 128, 4096), (40, 8, 8, 64, 1500), (300, 4, 1, 32, 1200), (20, 8, 4, 64, 5000)])
+def test_a_sequence_has_its_bits_wherever_it_stands_in_the_batch(b, h, g, d, most):
+    # Sequences are taken by length, in order, or in chunks: again, and in another order, each gives the same bits.
+    _say("attention, order of the batch", b, g, d)
+    rng = np.random.default_rng(b + d)
+    lens = rng.integers(1, most + 1, b)
+    lens[0] = most
+    q, kn, vn, ks, vs, table, lens, scale = _attention_case(rng, b, h, g, d, 16, lens)
+    first = _attend(q, kn, vn, ks, vs, table, lens, scale)
+    for _ in range(3):
+        at = rng.permutation(b)
+        np.testing.assert_array_equal(_attend(q[at], kn, vn, ks, vs, table[at], lens[at], scale), first[at])
+        np.testing.assert_array_equal(_attend(q, kn, vn, ks, vs, table, lens, scale), first)
